@@ -14,6 +14,8 @@ LIB_PATH = os.path.join(HERE, "libds_ocr_hip.so")
 
 ROUTE_DECODE = 0
 ROUTE_CFG = 1
+KV_F32 = 0
+KV_BF16 = 1
 
 f32p = np.ctypeslib.ndpointer(dtype=np.float32, flags="C_CONTIGUOUS")
 u16p = np.ctypeslib.ndpointer(dtype=np.uint16, flags="C_CONTIGUOUS")
@@ -26,6 +28,12 @@ class Int4Block(C.Structure):
     """ds_int4_block_t (include/ds_quantize.h)."""
     _fields_ = [("qweight", vp), ("scale", vp), ("offset", vp), ("out_dim", C.c_int), ("in_dim", C.c_int),
                 ("bytes", C.c_size_t)]
+
+
+class KvCache(C.Structure):
+    """ds_hip_kv_t (include/ds_hip.h): K and V rows in device memory, strides in elements."""
+    _fields_ = [("k", vp), ("v", vp), ("row_stride", C.c_int64), ("head_stride", C.c_int64), ("rows", C.c_int),
+                ("n_heads", C.c_int), ("head_dim", C.c_int), ("dtype", C.c_int)]
 
 
 # name -> (restype, argtypes); the exported C-ABI surface.
@@ -125,6 +133,15 @@ SIGNATURES = {
     "ds_hip_attn_kv": (C.c_int, [vp, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_int)]),
     "ds_hip_attn_load_kv": (C.c_int, [vp, vp, vp, C.c_int, C.c_int]),
     "ds_hip_attn_forward": (C.c_int, [vp, vp, vp, vp, C.c_int]),
+    "ds_hip_attn_kv_view": (C.c_int, [vp, C.POINTER(KvCache)]),
+    "ds_hip_tree_attention": (C.c_int, [vp, C.c_int64, vp, vp, C.c_int64, vp, C.c_int64, C.c_int, C.POINTER(KvCache),
+                                        C.c_int, C.POINTER(KvCache), vp, C.c_int, C.c_float, C.c_int, C.c_int]),
+    "ds_hip_tree_verify": (C.c_int, [vp, vp, vp, C.c_int64, vp, C.c_int64, C.c_int, vp, vp, C.c_int, vp]),
+    "ds_hip_tree_verify_greedy": (C.c_int, [vp, vp, vp, vp, vp, C.c_int]),
+    "ds_hip_tree_commit": (C.c_int, [C.POINTER(KvCache), C.c_int, C.POINTER(KvCache), C.c_int, vp, vp, vp, C.c_int64, vp,
+                                     C.c_int, vp, vp, C.c_int64, vp, C.c_int64, C.c_int]),
+    "ds_hip_kv_evict": (C.c_int, [C.POINTER(KvCache), C.c_int, C.c_int, vp, C.c_int64, vp, C.c_int64, vp, C.c_int64, vp,
+                                  C.c_int64, C.c_int, C.c_int, vp]),
     "ds_hip_stack_set_attention": (C.c_int, [vp, vp, C.c_int, vp, C.c_float, C.c_int, C.c_int]),
     "ds_hip_stack_set_sampling": (C.c_int, [vp, C.c_float, C.c_int, C.c_int]),
     "ds_hip_lm_head_sample": (C.c_int, [vp, vp, C.c_int, C.c_int, vp, C.c_int, C.c_float, C.c_int, vp]),

@@ -365,6 +365,50 @@ hipError_t dsh_launch_dec_layer(const dsh_layer_t *L, const dsh_split_t *F, cons
 /* out = Σ copies of X ([copies][H]); clears X and zero_p[0..zero_n). */
 hipError_t dsh_launch_dec_copy_sum(float *X, int H, float *out, float *zero_p, int zero_n, hipStream_t s);
 
+/* ---- drafted tokens over a KV cache (k_tree.hip, k_evict.hip) ---- */
+#define DSH_TREE_MAX 128
+typedef struct {
+  void *k, *v;
+  int64_t row_stride, head_stride; /* elements */
+  int n_heads, head_dim, bf16;
+} dsh_kv_t;
+typedef struct {
+  dsh_kv_t cache, tree;
+  const float *q;
+  const int *parents;
+  float *out, *lse, *scores; /* lse, scores: optional */
+  int64_t q_stride, out_stride, score_stride;
+  int n_cache, n_nodes, n_heads, prefill_len, window;
+  float scale;
+} dsh_tree_attn_t;
+hipError_t dsh_launch_tree_attention(const dsh_tree_attn_t *A, hipStream_t s);
+/* target: greedy (p, q, u unused); else p, optionally q, and u. */
+hipError_t dsh_launch_tree_verify(int *path, int *result, const float *p, int64_t p_stride, const float *q,
+                                  int64_t q_stride, int vocab, const int *target, const int *tokens, const int *parents,
+                                  int n_nodes, const float *u, hipStream_t s);
+typedef struct {
+  dsh_kv_t cache, tree;
+  const int *path, *result;
+  const float *scores, *lse, *acc; /* acc NULL: no weights */
+  float *acc_out;
+  int *pos; /* optional */
+  int64_t score_stride, acc_stride, pos_stride;
+  int n_cache, n_nodes, n_heads, pos0;
+} dsh_tree_commit_t;
+hipError_t dsh_launch_tree_commit(const dsh_tree_commit_t *A, hipStream_t s);
+typedef struct {
+  dsh_kv_t cache;
+  const float *acc;
+  const int *pos; /* optional */
+  float *acc_out; /* optional, like pos_out and slots */
+  int *pos_out, *slots;
+  int64_t acc_stride, acc_out_stride, pos_stride, pos_out_stride;
+  int n, keep, sink, recent_from;
+  int *work; /* dsh_kv_evict_work ints */
+} dsh_kv_evict_t;
+size_t dsh_kv_evict_work(int n_heads, int n, int keep);
+hipError_t dsh_launch_kv_evict(const dsh_kv_evict_t *A, hipStream_t s);
+
 #ifdef __cplusplus
 }
 #endif

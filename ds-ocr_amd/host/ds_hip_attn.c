@@ -181,6 +181,11 @@ int ds_hip_attn_hidden(const ds_hip_attn_t *A) { return A ? A->d.H : 0; }
 
 int ds_hip_attn_max_seq(const ds_hip_attn_t *A) { return A ? A->d.max_seq : 0; }
 
+void ds_hip_attn_heads(const ds_hip_attn_t *A, int *n_heads, int *head_dim) {
+  *n_heads = A->d.n_heads;
+  *head_dim = A->d.head_dim;
+}
+
 size_t ds_hip_attn_weight_bytes(const ds_hip_attn_t *A) {
   return A ? (size_t)4 * A->d.H * A->d.n_heads * A->d.head_dim * 2 + (size_t)2 * A->d.H * 4 : 0;
 }

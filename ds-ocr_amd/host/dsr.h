@@ -39,7 +39,7 @@ int dsr_derr_check(void);
 dsh_rcert_t dsr_rcert(int tag);
 
 /* Grow-only device staging buffer per slot (not thread-safe, like the reference API). */
-enum { DSR_SLOT_X, DSR_SLOT_Y, DSR_SLOT_A, DSR_SLOT_B, DSR_SLOT_C, DSR_SLOT_D, DSR_SLOT_IDX, DSR_SLOT_PF, DSR_SLOT_XC, DSR_NSLOTS };
+enum { DSR_SLOT_X, DSR_SLOT_Y, DSR_SLOT_A, DSR_SLOT_B, DSR_SLOT_C, DSR_SLOT_D, DSR_SLOT_IDX, DSR_SLOT_PF, DSR_SLOT_XC, DSR_SLOT_TREE, DSR_NSLOTS };
 void *dsr_scratch(int slot, size_t bytes);
 
 /* The per-function path's one-launch expert kernels: the device buffer of epoch-tagged h words (at
@@ -105,6 +105,7 @@ hipError_t ds_hip_attn_enqueue(const struct ds_hip_attn *A, const float *x_in, c
                                const float *WrT_next, int E_next, float *partials_next, int threads);
 int ds_hip_attn_hidden(const struct ds_hip_attn *A);
 int ds_hip_attn_max_seq(const struct ds_hip_attn *A); /* KV positions the caches hold */
+void ds_hip_attn_heads(const struct ds_hip_attn *A, int *n_heads, int *head_dim);
 size_t ds_hip_attn_weight_bytes(const struct ds_hip_attn *A); /* projections and norms read per token */
 
 #endif

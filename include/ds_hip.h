@@ -253,6 +253,98 @@ int ds_hip_attn_load_kv(ds_hip_attn_t *A, const float *k_host, const float *v_ho
  * n_dev = RMSNorm(h) (device [hidden] each). Asynchronous. */
 int ds_hip_attn_forward(ds_hip_attn_t *A, float *h_dev, float *n_dev, const float *x_dev, int pos);
 
+/* ---------------- drafted tokens over a KV cache (speculative decoding) ---------------- */
+/* No counterpart in the reference, whose decoder runs one token per step. A step drafts a tree of tokens, runs all of
+ * its nodes through the model at once, keeps the path that the target model's probabilities accept, and may keep the
+ * cache within a budget by dropping the rows that attention used least:
+ *   per layer  ds_hip_tree_attention   the nodes' attention over the cached rows and their own ancestors
+ *   once       ds_hip_tree_verify      the accepted path and the token after it (or ds_hip_tree_verify_greedy)
+ *   per layer  ds_hip_tree_commit      the accepted nodes' K and V rows into the cache, their weights onto the rows'
+ *   at need    ds_hip_kv_evict         per head the n_keep rows that stay
+ * All four take device pointers, run asynchronously on the library's stream, on device 0 whatever the caller's current
+ * device is, and keep nothing between calls but a grow-only workspace. Outputs must not overlap inputs unless said.
+ *
+ * The tree: parents_dev[i] of n_nodes (at most DS_HIP_TREE_MAX_NODES) is -1 for a child of the last committed token, or
+ * the index j < i of another node. Any other value makes node i a padding node, and so is every node below one: it
+ * sees nothing, is never accepted, and its inputs may hold anything. Node i stands at position n_cache + depth(i) (depth
+ * 0 below the committed token). */
+#define DS_HIP_TREE_MAX_NODES 128
+enum { DS_HIP_KV_F32 = 0, DS_HIP_KV_BF16 = 1 };
+/* K and V rows in device memory: row r of head h starts at element r * row_stride + h * head_stride of k and of v. k, v
+ * and both strides (in bytes) are multiples of 16; rows do not overlap. head_dim: 64, 128, 192 or 256. k rows are roped. */
+typedef struct {
+  void *k, *v;
+  int64_t row_stride, head_stride;
+  int rows;     /* rows that the arrays hold */
+  int n_heads;  /* key/value heads */
+  int head_dim;
+  int dtype;    /* DS_HIP_KV_* */
+} ds_hip_kv_t;
+/* The cache of an attention handle in this form (f32, max_seq rows). Host only. */
+int ds_hip_attn_kv_view(const ds_hip_attn_t *A, ds_hip_kv_t *kv);
+
+/* Attention of n_nodes drafted tokens: query head h of node i over head h / (n_heads / cache->n_heads) of the cached
+ * rows [0, n_cache) and of the tree's rows (row i of tree: node i's own K and V, of the cache's type and shape) of i and
+ * its ancestors. With s = scale * q.k over what node i sees: lse = log(sum(exp(s))), out = sum(exp(s - lse) v), with
+ * the true exponential (ds_hip_attn_forward's is the reference's ds_fast_expf). window > 0 (ds_hip_attn_set_window's
+ * R-SWA): a node at a position >= prefill_len sees the positions below prefill_len and the last `window` ones, itself
+ * among them; row r of the cache is then position r. A node that sees nothing gets out 0 and lse -inf.
+ * q_dev, out_dev: f32 [n_nodes][n_heads * head_dim], rows q_stride and out_stride floats apart (multiples of 4, 16-byte
+ * aligned). lse_dev (optional): [n_heads][n_nodes]. scores_dev (optional): s as [n_heads][n_nodes][score_stride], cached
+ * rows at 0..n_cache-1, nodes at n_cache..n_cache+n_nodes-1, -inf where node i does not see; for ds_hip_tree_commit.
+ * What a node does not see may hold anything, NaN and infinities included; a value that is not finite in what it sees
+ * makes its head's output not finite. n_cache 0 is allowed (cache->k and v may then be NULL). */
+int ds_hip_tree_attention(float *out_dev, int64_t out_stride, float *lse_dev, float *scores_dev, int64_t score_stride,
+                          const float *q_dev, int64_t q_stride, int n_heads, const ds_hip_kv_t *cache, int n_cache,
+                          const ds_hip_kv_t *tree, const int *parents_dev, int n_nodes, float scale, int prefill_len,
+                          int window);
+
+/* Verification against the target's probabilities. p_dev: f32 [n_nodes + 1][p_stride], row 0 the target's distribution
+ * after the last committed token, row 1 + i the one after node i; q_dev: the distributions that the drafts were drawn
+ * from, row 0 for the root's children and row 1 + i for node i's (children of one context are independent draws of its
+ * row), or NULL when drafts were chosen without randomness (a lookup, a top-k). u_dev: n_nodes + 1 numbers of [0, 1).
+ * From the root on, a context's children are tried in ascending order, and the first accepted one is the next context:
+ *   q given: r = max(p - c q, 0) at the child's token, accepted if r > 0 and u[i] q Z < r, with c = 0 and Z = 1 at first;
+ *            a rejection adds Z to c and makes Z the sum of max(p - c q, 0) (repeated norm(max(p - q, 0)));
+ *   q NULL:  r = p at the token (0 if a sibling before it had the same), accepted if r > 0 and u[i] (1 - the sum of the
+ *            siblings' r before it) < r.
+ * Where no child is accepted, the step's token is drawn from what is left, w = max(p - c q, 0), or p without the rejected
+ * tokens (p itself if nothing is left): the smallest v with w[v] > 0 and w[0] + ... + w[v] > u[n_nodes] * sum(w); -1 if
+ * p holds nothing positive. Sums and products are in 64 bits. Tokens outside [0, vocab) are rejected; a value of p or q
+ * that is not positive and finite counts as 0. path_dev[n_nodes]: the accepted nodes, then -1; result_dev[2]: their
+ * number and the token. n_nodes 0 (tokens and parents may be NULL) draws a token from p. */
+int ds_hip_tree_verify(int *path_dev, int *result_dev, const float *p_dev, int64_t p_stride, const float *q_dev,
+                       int64_t q_stride, int vocab, const int *tokens_dev, const int *parents_dev, int n_nodes,
+                       const float *u_dev);
+/* The same for greedy decoding: target_dev[0] is the target's token after the last committed one, target_dev[1 + i]
+ * after node i (its argmax after whatever sampling rules); a child is accepted if it is its context's target, and the
+ * step's token is the last context's target. */
+int ds_hip_tree_verify_greedy(int *path_dev, int *result_dev, const int *target_dev, const int *tokens_dev,
+                              const int *parents_dev, int n_nodes);
+
+/* The accepted nodes (path_dev and result_dev[0] of a verification; entries outside [0, n_nodes) and all behind the first of
+ * them are left out) go to the rows n_cache, n_cache + 1, ... of the cache, which must hold n_cache + n_nodes rows. acc
+ * (optional; [cache->n_heads][acc_stride], acc_stride >= n_cache + n_nodes): every row's attention weight so far; with
+ * ds_hip_tree_attention's scores and lse of n_heads query heads,
+ *   acc_out[g][j] = acc[g][j] + sum over accepted i and the heads h of g of exp(s[h][i][j] - lse[h][i]), j < n_cache,
+ * and the accepted nodes' own sums for their new rows. acc_out may be acc itself. pos_dev (optional;
+ * [cache->n_heads][pos_stride]): the new rows' entries become pos0, pos0 + 1, ... Rows and entries behind the accepted
+ * ones are left as they were. */
+int ds_hip_tree_commit(const ds_hip_kv_t *cache, int n_cache, const ds_hip_kv_t *tree, int n_nodes, const int *path_dev,
+                       const int *result_dev, const float *scores_dev, int64_t score_stride, const float *lse_dev,
+                       int n_heads, const float *acc_dev, float *acc_out_dev, int64_t acc_stride, int *pos_dev,
+                       int64_t pos_stride, int pos0);
+
+/* Keeps n_keep of n_rows rows of every head, in rows 0..n_keep-1: the rows with the lowest acc go, the lower row first
+ * among equal ones (a NaN counts as -inf); rows with pos < sink or pos >= recent_from go only when no others are left
+ * (pos NULL: the row number). The kept rows from n_keep on move, in order, into the evicted ones below n_keep, in order;
+ * no other row is written. slots_dev (optional, [n_heads][n_keep]): the row that each one was. acc_out and pos_out
+ * (optional) are acc and pos of the rows that stay; each may be its input itself (with the same stride). The positions of
+ * a cache that has evicted are in no order, so that attention over it takes no window. */
+int ds_hip_kv_evict(const ds_hip_kv_t *cache, int n_rows, int n_keep, const float *acc_dev, int64_t acc_stride,
+                    float *acc_out_dev, int64_t acc_out_stride, const int *pos_dev, int64_t pos_stride, int *pos_out_dev,
+                    int64_t pos_out_stride, int sink, int recent_from, int *slots_dev);
+
 /* ---------------- decode stack: n MoE layers + argmax LM head ---------------- */
 typedef struct ds_hip_stack ds_hip_stack_t;
 
