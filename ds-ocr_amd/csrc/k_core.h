@@ -381,7 +381,8 @@ typedef struct {
   int n_cache, n_nodes, n_heads, prefill_len, window;
   float scale;
 } dsh_tree_attn_t;
-hipError_t dsh_launch_tree_attention(const dsh_tree_attn_t *A, hipStream_t s);
+size_t dsh_tree_attention_work(const dsh_tree_attn_t *A); /* floats */
+hipError_t dsh_launch_tree_attention(const dsh_tree_attn_t *A, float *work, hipStream_t s);
 /* target: greedy (p, q, u unused); else p, optionally q, and u. */
 hipError_t dsh_launch_tree_verify(int *path, int *result, const float *p, int64_t p_stride, const float *q,
                                   int64_t q_stride, int vocab, const int *target, const int *tokens, const int *parents,

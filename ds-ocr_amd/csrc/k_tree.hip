@@ -3,6 +3,10 @@
 #include "dsh.h"
 #include "k_core.h"
 
+#include <string.h>
+
+#include <type_traits>
+
 typedef unsigned long long u64;
 
 // ---------------------------------------------------------------------------- the tree
@@ -54,72 +58,409 @@ __device__ __forceinline__ bool tree_in_window(int p, int pos, int prefill_len, 
 }
 
 // ---------------------------------------------------------------------------- attention
-template <bool BF>
-__device__ __forceinline__ float kv_at(const void *p, int64_t i) {
-  return BF ? dsh_bf16_to_f32(((const uint16_t *)p)[i]) : ((const float *)p)[i];
+// The rows of one key head are the (node, query head of its group) pairs, row r node r % n_nodes of head r / n_nodes. A wave
+// owns 16 rows and goes over tiles of AT positions with a running maximum and sum, everything in registers:
+//   S^T[position][row] = K Q^T: lane (i, g), i = lane & 15, g = lane >> 4, has row i of the K tile as the product's left
+//   operand, and gets back row i of the queries at the positions 4g..4g+3 of a 16-position subtile;
+//   O^T[dimension][row] += V^T P^T: that is just the right operand of the second product, whose summation index the lanes'
+//   g and the four positions are. The order of the dimensions within a product and of its rows is free, so K and V are
+//   loaded as they lie in memory: 16 bytes a lane, whole lines, no LDS and no exchange between lanes.
+// The maximum is only moved, and the sums scaled, when some score exceeds it by ATT_SLACK: weights stay below exp(ATT_SLACK).
+//   f32 cache: v_mfma_f32_16x16x4, exact products and f32 sums. bf16 cache: v_mfma_f32_16x16x32_bf16, the f32 queries and
+//   weights in three bf16 parts each that add up to them exactly (24 bits), so that only the f32 sums round.
+#define ATT_SLACK 10.0f
+#define ATT_L2E 1.44269504088896340736f
+
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// How a launch cuts the work; a tile is AT positions of the cache (tiles in [gap, gap + skip) are seen by no node and left out)
+// or of the tree.
+struct attend_plan {
+  int tile_rows, pos_waves;  // 16-row tiles and shares of the positions in a block: a wave each
+  int groups, splits;        // blocks per key head: groups of tile_rows tiles of rows, splits of the tiles of positions
+  int cache_tiles, tree_tiles, gap, skip;
+  float *part, *ml;          // [head][group][split][16 * tile_rows] x D, and the maximum and sum
+};
+
+__device__ __forceinline__ float att_exp(float x) { return __builtin_amdgcn_exp2f(x * ATT_L2E); }
+
+// x as three bf16 numbers whose sum it is (each the upper half of what is left: 8 + 8 + 8 bits), in the upper halves.
+__device__ __forceinline__ void split3(float x, uint32_t &a, uint32_t &b, uint32_t &c) {
+  a = __float_as_uint(x) & 0xFFFF0000u;
+  const float r = x - __uint_as_float(a);
+  b = __float_as_uint(r) & 0xFFFF0000u;
+  c = __float_as_uint(r - __uint_as_float(b));
+}
+// The upper halves of lo and hi, side by side.
+__device__ __forceinline__ uint32_t upper2(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+
+template <int D>
+struct frag_f32 {
+  static constexpr int AT = 16, NB = D / 16;
+  f32x4 q[NB], k[NB], v[4][D / 64];
+  __device__ __forceinline__ void load_q(const float *p, int g) {
+#pragma unroll
+    for (int b = 0; b < NB; b++) q[b] = *(const f32x4 *)(p + 16 * b + 4 * g);
+  }
+  // row(x): element offset of the tile's position x
+  template <typename R>
+  __device__ __forceinline__ void load_k(const void *base, R row, int i, int g) {
+    const float *p = (const float *)base + row(i) + 4 * g;
+#pragma unroll
+    for (int b = 0; b < NB; b++) k[b] = *(const f32x4 *)(p + 16 * b);
+  }
+  template <typename R>
+  __device__ __forceinline__ void load_v(const void *base, R row, int i, int g) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const float *p = (const float *)base + row(4 * g + r) + 4 * i;
+#pragma unroll
+      for (int b = 0; b < D / 64; b++) v[r][b] = *(const f32x4 *)(p + 64 * b);
+    }
+  }
+  __device__ __forceinline__ void scores(float *s) const {
+    f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f}, c = a;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[b][e], q[b][e], a, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(k[b][e + 1], q[b][e + 1], c, 0, 0, 0);
+      }
+#pragma unroll
+    for (int r = 0; r < 4; r++) s[r] = a[r] + c[r];
+  }
+  __device__ __forceinline__ void add(const float *p, f32x4 *o) const {
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int b = 0; b < D / 64; b++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) o[4 * b + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][b][t], p[r], o[4 * b + t], 0, 0, 0);
+  }
+  // Whether position x of the lane's (4g + x) holds a value that is not finite here; and takes it out.
+  __device__ __forceinline__ bool clean_v(int x) {
+    bool bad = false;
+#pragma unroll
+    for (int b = 0; b < D / 64; b++)
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+        if (!(__builtin_fabsf(v[x][b][t]) < __builtin_huge_valf())) {
+          bad = true;
+          v[x][b][t] = 0.0f;
+        }
+    return bad;
+  }
+  // Dimension of o[4b + t][r].
+  static __device__ __forceinline__ int dim(int b, int r, int g) { return 64 * b + 16 * g + 4 * r; }
+};
+
+// Output in registers: o[4b + t][r] is dimension dim(b, r, g) + t of the lane's row.
+template <int D>
+struct frag_bf16 {
+  static constexpr int AT = 32, NS = D / 32;
+  u32x4 q[3][NS], k[2][NS];
+  uint32_t v[8][D / 32];  // position 16 (x >> 2) + 4g + (x & 3), D / 64 groups of four dimensions
+  __device__ __forceinline__ void load_q(const float *p, int g) {
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+      const f32x4 x0 = *(const f32x4 *)(p + 32 * s + 8 * g), x1 = *(const f32x4 *)(p + 32 * s + 8 * g + 4);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        uint32_t a[2], b[2], c[2];
+        split3(e < 2 ? x0[2 * e] : x1[2 * e - 4], a[0], b[0], c[0]);
+        split3(e < 2 ? x0[2 * e + 1] : x1[2 * e - 3], a[1], b[1], c[1]);
+        q[0][s][e] = upper2(a[0], a[1]);
+        q[1][s][e] = upper2(b[0], b[1]);
+        q[2][s][e] = upper2(c[0], c[1]);
+      }
+    }
+  }
+  template <typename R>
+  __device__ __forceinline__ void load_k(const void *base, R row, int i, int g) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint16_t *p = (const uint16_t *)base + row(16 * h + i) + 8 * g;
+#pragma unroll
+      for (int s = 0; s < NS; s++) k[h][s] = *(const u32x4 *)(p + 32 * s);
+    }
+  }
+  template <typename R>
+  __device__ __forceinline__ void load_v(const void *base, R row, int i, int g) {
+#pragma unroll
+    for (int x = 0; x < 8; x++) {
+      const uint16_t *p = (const uint16_t *)base + row(16 * (x >> 2) + 4 * g + (x & 3)) + 4 * i;
+#pragma unroll
+      for (int b = 0; b < D / 64; b++) {
+        const uint2 w = *(const uint2 *)(p + 64 * b);
+        v[x][2 * b] = w.x;
+        v[x][2 * b + 1] = w.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void scores(float *s) const {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int l = 2; l >= 0; l--)  // the small parts first
+#pragma unroll
+        for (int x = 0; x < NS; x++)
+          a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[h][x]), __builtin_bit_cast(bf16x8, q[l][x]),
+                                                      a, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; r++) s[4 * h + r] = a[r];
+    }
+  }
+  __device__ __forceinline__ void add(const float *p, f32x4 *o) const {
+    u32x4 w[3];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      uint32_t a[2], b[2], c[2];
+      split3(p[2 * e], a[0], b[0], c[0]);
+      split3(p[2 * e + 1], a[1], b[1], c[1]);
+      w[0][e] = upper2(a[0], a[1]);
+      w[1][e] = upper2(b[0], b[1]);
+      w[2][e] = upper2(c[0], c[1]);
+    }
+#pragma unroll
+    for (int b = 0; b < D / 64; b++)
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        u32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint32_t lo = v[2 * e][2 * b + (t >> 1)], hi = v[2 * e + 1][2 * b + (t >> 1)];
+          x[e] = __builtin_amdgcn_perm(hi, lo, t & 1 ? 0x07060302u : 0x05040100u);
+        }
+#pragma unroll
+        for (int l = 2; l >= 0; l--)
+          o[4 * b + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, w[l]),
+                                                                 o[4 * b + t], 0, 0, 0);
+      }
+  }
+  __device__ __forceinline__ bool clean_v(int x) {
+    bool bad = false;
+#pragma unroll
+    for (int b = 0; b < D / 32; b++) {
+      if ((v[x][b] & 0x7F80u) == 0x7F80u) bad = true, v[x][b] &= 0xFFFF0000u;
+      if ((v[x][b] & 0x7F800000u) == 0x7F800000u) bad = true, v[x][b] &= 0xFFFFu;
+    }
+    return bad;
+  }
+  static __device__ __forceinline__ int dim(int b, int r, int g) { return 64 * b + 16 * g + 4 * r; }
+};
+
+// A block: tile_rows x pos_waves waves over one split of the tiles of one key head; the waves of a row tile put their sums
+// together, and the block writes them for k_tree_join (splits > 1) or finishes its rows itself.
+template <int D, bool BF, int W>
+__global__ void __launch_bounds__(64 * W) k_tree_attend(dsh_tree_attn_t A, attend_plan P) {
+  typedef typename std::conditional<BF, frag_bf16<D>, frag_f32<D>>::type frag;
+  constexpr int AT = frag::AT, NV = AT / 4;  // scores a lane
+  __shared__ tree_lds t;
+  __shared__ float s_m[W][16], s_l[W][16];
+  extern __shared__ __attribute__((aligned(16))) float s_o[];  // [pos_waves - 1][tile_rows][16][D]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int G = A.cache.n_heads, grp = A.n_heads / G, T = A.n_nodes, R = T * grp;
+  const int kh = blockIdx.y, z = blockIdx.z, split = blockIdx.x;
+  const int rt = wave % P.tile_rows, pw = wave / P.tile_rows;
+  const int row = 16 * (z * P.tile_rows + rt) + i;  // the lane's
+  const int rr = min(row, R - 1), node = rr % T, head = kh * grp + rr / T;
+  const int tiles = P.cache_tiles - P.skip + P.tree_tiles;
+  const int per = (tiles + P.splits - 1) / P.splits, t0 = split * per, t1 = min(t0 + per, tiles);
+  frag F;
+  F.load_q(A.q + node * A.q_stride + (int64_t)head * D, g);
+  // what only the tree's own tiles, a window, scores and whole rows need
+  const bool need = P.splits == 1 || A.scores || A.window > 0 || t1 > P.cache_tiles - P.skip;
+  if (need) tree_ancestors(t, A.parents, T);
+  const u64 anc0 = need ? t.anc[node][0] : 0, anc1 = need ? t.anc[node][1] : 0;
+  const bool live = !need || (anc0 | anc1);
+  const int pos = A.n_cache + __popcll(anc0) + __popcll(anc1) - 1;
+  const float inf = __builtin_huge_valf();
+  float m = -inf, l = 0.0f, ml2 = 0.0f;
+  f32x4 o[D / 16];
+#pragma unroll
+  for (int b = 0; b < D / 16; b++) o[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float *sc = A.scores ? A.scores + ((int64_t)head * T + node) * A.score_stride : nullptr;
+
+  for (int tile = t0 + pw; tile < t1; tile += P.pos_waves) {
+    int x = tile >= P.gap ? tile + P.skip : tile;
+    const bool own = x >= P.cache_tiles;
+    const dsh_kv_t &c = own ? A.tree : A.cache;
+    const int p0 = AT * (own ? x - P.cache_tiles : x), end = own ? T : A.n_cache;
+    const auto at = [&](int k) { return (int64_t)min(p0 + k, end - 1) * c.row_stride + kh * c.head_stride; };
+    F.load_k(c.k, at, i, g);
+    F.load_v(c.v, at, i, g);
+    float s[NV];
+    F.scores(s);
+#pragma unroll
+    for (int k = 0; k < NV; k++) s[k] *= A.scale;
+    bool part = !live || p0 + AT > end || own || A.window > 0;
+    if (__any(part)) {  // some position is not seen by some row
+      uint32_t seen = 0;
+#pragma unroll
+      for (int k = 0; k < NV; k++) {
+        const int j = p0 + 16 * (k >> 2) + 4 * g + (k & 3);
+        bool see = live && j < end;
+        if (own) {
+          const int a = min(j, DSH_TREE_MAX - 1);
+          see = see && (((a < 64 ? anc0 >> a : anc1 >> (a - 64)) & 1) != 0);
+          if (A.window > 0 && see) see = tree_in_window(A.n_cache + tree_depth(t.anc[a]), pos, A.prefill_len, A.window);
+        } else {
+          see = see && tree_in_window(j, pos, A.prefill_len, A.window);
+        }
+        s[k] = see ? s[k] : -inf;
+        seen |= (uint32_t)see << k;
+      }
+      // A weight of 0 does not take out a V that is not finite: such rows are set to 0, and what sees them to NaN.
+      bool poison = false;
+#pragma unroll
+      for (int k = 0; k < NV; k++) {
+        const u64 bad = __ballot(F.clean_v(k));
+        poison |= ((bad >> (16 * g)) & 0xFFFF) && ((seen >> k) & 1);
+      }
+      if (__any(poison)) {
+        int y = poison;
+        y |= __shfl_xor(y, 16);
+        y |= __shfl_xor(y, 32);
+        if (y)
+#pragma unroll
+          for (int b = 0; b < D / 16; b++) o[b] += __builtin_nanf("");
+      }
+    }
+    if (sc && row < R) {
+#pragma unroll
+      for (int k = 0; k < NV; k++) {
+        const int j = p0 + 16 * (k >> 2) + 4 * g + (k & 3);
+        if (j < end) sc[own ? (int64_t)A.n_cache + j : j] = s[k];
+      }
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int k = 1; k < NV; k++) mx = fmaxf(mx, s[k]);
+    if (__any(mx > m + ATT_SLACK)) {
+      mx = fmaxf(mx, m);
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float f = mx == m ? 1.0f : att_exp(m - mx);
+      m = mx;
+      ml2 = m == -inf ? 0.0f : m * ATT_L2E;
+      l *= f;
+#pragma unroll
+      for (int b = 0; b < D / 16; b++) o[b] *= f;
+    }
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+      s[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], ATT_L2E, -ml2));
+      l += s[k];
+    }
+    F.add(s, o);
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+
+  if (P.pos_waves > 1) {
+    if (g == 0) {
+      s_m[wave][i] = m;
+      s_l[wave][i] = l;
+    }
+    __syncthreads();
+    float M = -inf;
+    for (int w = 0; w < P.pos_waves; w++) M = fmaxf(M, s_m[w * P.tile_rows + rt][i]);
+    l = 0.0f;
+    for (int w = 0; w < P.pos_waves; w++) {
+      const float mw = s_m[w * P.tile_rows + rt][i];
+      l += s_l[w * P.tile_rows + rt][i] * (mw == M ? 1.0f : att_exp(mw - M));
+    }
+    const float f = m == M ? 1.0f : att_exp(m - M);
+    m = M;
+#pragma unroll
+    for (int b = 0; b < D / 16; b++) o[b] *= f;
+    if (pw > 0) {
+      float *d = s_o + (((pw - 1) * P.tile_rows + rt) * 16 + i) * D;
+#pragma unroll
+      for (int b = 0; b < D / 64; b++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          *(f32x4 *)(d + frag::dim(b, r, g)) = f32x4{o[4 * b][r], o[4 * b + 1][r], o[4 * b + 2][r], o[4 * b + 3][r]};
+    }
+    __syncthreads();
+    if (pw > 0) return;
+    for (int w = 0; w < P.pos_waves - 1; w++) {
+      const float *d = s_o + ((w * P.tile_rows + rt) * 16 + i) * D;
+#pragma unroll
+      for (int b = 0; b < D / 64; b++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const f32x4 y = *(const f32x4 *)(d + frag::dim(b, r, g));
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[4 * b + e][r] += y[e];
+        }
+    }
+  }
+  if (row >= R) return;
+  float *to;
+  float f = 1.0f;
+  if (P.splits == 1) {
+    to = A.out + node * A.out_stride + (int64_t)head * D;
+    f = !live || l == 0.0f ? 0.0f : 1.0f / l;
+    if (A.lse && g == 0) A.lse[(int64_t)head * T + node] = f == 0.0f ? -inf : m + logf(l);
+  } else {
+    const int64_t at = (((int64_t)kh * P.groups + z) * P.splits + split) * 16 * P.tile_rows + 16 * rt + i;
+    to = P.part + at * D;
+    if (g == 0) {
+      P.ml[2 * at] = m;
+      P.ml[2 * at + 1] = l;
+    }
+  }
+  const bool zero = P.splits == 1 && (!live || l == 0.0f);
+#pragma unroll
+  for (int b = 0; b < D / 64; b++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      f32x4 y = f32x4{o[4 * b][r], o[4 * b + 1][r], o[4 * b + 2][r], o[4 * b + 3][r]} * f;
+      if (zero) y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      *(f32x4 *)(to + frag::dim(b, r, g)) = y;
+    }
 }
 
-// One block per node and query head: every wave runs the softmax over its share of the positions with a running maximum
-// and sum, the lanes over the head's dimensions, and the waves' results are put together at the end.
-template <int D, bool BF>
-__global__ void __launch_bounds__(256) k_tree_attend(dsh_tree_attn_t A) {
-  constexpr int E = D / 64;
+// The splits of one row put together, in their order: a block of D threads per row, the maxima and sums by its first wave.
+template <int D>
+__global__ void __launch_bounds__(256) k_tree_join(dsh_tree_attn_t A, attend_plan P) {
   __shared__ tree_lds t;
-  __shared__ float s_o[4][D], s_m[4], s_l[4];
-  const int i = blockIdx.x, h = blockIdx.y, kh = h / (A.n_heads / A.cache.n_heads);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  tree_ancestors(t, A.parents, A.n_nodes);
-  const bool live = t.anc[i][0] | t.anc[i][1];
-  const int pos = A.n_cache + tree_depth(t.anc[i]);
-  float q[E], o[E], m = -__builtin_huge_valf(), l = 0.0f;
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    q[e] = A.q[i * A.q_stride + (int64_t)h * D + lane + 64 * e];
-    o[e] = 0.0f;
-  }
-  float *sc = A.scores ? A.scores + ((int64_t)h * A.n_nodes + i) * A.score_stride : nullptr;
-  for (int j = wave; j < A.n_cache + A.n_nodes; j += 4) {
-    const bool own = j >= A.n_cache;
-    const int a = j - A.n_cache;
-    bool see = live && (!own || tree_bit(t.anc[i], a));
-    see = see && tree_in_window(own ? A.n_cache + tree_depth(t.anc[a]) : j, pos, A.prefill_len, A.window);
-    float s = -__builtin_huge_valf();
-    if (see) {
-      const dsh_kv_t &c = own ? A.tree : A.cache;
-      const int64_t at = (own ? a : j) * c.row_stride + kh * c.head_stride;
-      float d = 0.0f;
-#pragma unroll
-      for (int e = 0; e < E; e++) d = __builtin_fmaf(q[e], kv_at<BF>(c.k, at + lane + 64 * e), d);
-      s = dsh_wave_sum(d) * A.scale;
-      const float mn = fmaxf(m, s), f = mn == m ? 1.0f : expf(m - mn), w = mn == s ? 1.0f : expf(s - mn);
-      l = l * f + w;
-#pragma unroll
-      for (int e = 0; e < E; e++) o[e] = o[e] * f + w * kv_at<BF>(c.v, at + lane + 64 * e);
-      m = mn;
+  __shared__ float s_f[1024], s_inv;
+  const int G = A.cache.n_heads, grp = A.n_heads / G, T = A.n_nodes;
+  const int row = blockIdx.x, kh = blockIdx.y, node = row % T, head = kh * grp + row / T;
+  const int z = row / (16 * P.tile_rows), in = row - z * 16 * P.tile_rows, stride = 16 * P.tile_rows;
+  const int64_t at = ((int64_t)kh * P.groups + z) * P.splits * stride + in;
+  tree_ancestors(t, A.parents, T);
+  const bool live = t.anc[node][0] | t.anc[node][1];
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    float M = -__builtin_huge_valf(), L = 0.0f;
+    for (int k = lane; k < P.splits; k += 64) M = fmaxf(M, P.ml[2 * (at + (int64_t)k * stride)]);
+    M = dsh_wave_max(M);
+    for (int k = lane; k < P.splits; k += 64) {
+      const float mk = P.ml[2 * (at + (int64_t)k * stride)], f = mk == M ? 1.0f : att_exp(mk - M);
+      s_f[k] = f;
+      L += f * P.ml[2 * (at + (int64_t)k * stride) + 1];
     }
-    if (sc && lane == 0) sc[j] = s;
-  }
-#pragma unroll
-  for (int e = 0; e < E; e++) s_o[wave][lane + 64 * e] = o[e];
-  if (lane == 0) {
-    s_m[wave] = m;
-    s_l[wave] = l;
+    L = dsh_wave_sum(L);
+    const bool none = !live || L == 0.0f;
+    if (lane == 0) {
+      s_inv = none ? 0.0f : 1.0f / L;
+      if (A.lse) A.lse[(int64_t)head * T + node] = none ? -__builtin_huge_valf() : M + logf(L);
+    }
   }
   __syncthreads();
-  const float M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  float f[4], L = 0.0f;
-#pragma unroll
-  for (int w = 0; w < 4; w++) {
-    f[w] = s_m[w] == M ? 1.0f : expf(s_m[w] - M);
-    L += f[w] * s_l[w];
-  }
-  for (int d = threadIdx.x; d < D; d += 256) {
-    float v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; w++) v += f[w] * s_o[w][d];
-    A.out[i * A.out_stride + (int64_t)h * D + d] = L == 0.0f ? 0.0f : v / L;
-  }
-  if (A.lse && threadIdx.x == 0) A.lse[(int64_t)h * A.n_nodes + i] = L == 0.0f ? -__builtin_huge_valf() : M + logf(L);
+  const int d = threadIdx.x;
+  if (d >= D) return;
+  float a = 0.0f;
+  const float *p = P.part + at * D + d;
+  for (int k = 0; k < P.splits; k++) a = __builtin_fmaf(s_f[k], p[(int64_t)k * stride * D], a);
+  A.out[node * A.out_stride + (int64_t)head * D + d] = s_inv == 0.0f ? 0.0f : a * s_inv;
 }
 
 // ---------------------------------------------------------------------------- verification
@@ -319,17 +660,70 @@ extern "C" {
       return hipErrorInvalidValue; \
   }
 
-hipError_t dsh_launch_tree_attention(const dsh_tree_attn_t *A, hipStream_t s) {
+// The cut of a launch's work. Row tiles: up to 8 (D <= 128; 4 beyond, whose registers need a whole SIMD) in a block, a wave each,
+// so that K and V come from the first-level cache for all but one of them; with fewer than 3 the rest of four waves share the
+// positions. Splits: as many as keep the card's 1024 SIMDs at two waves each, and no wave without a tile.
+static attend_plan attend_cut(const dsh_tree_attn_t *A) {
+  attend_plan P;
+  memset(&P, 0, sizeof P);
+  const int AT = A->cache.bf16 ? 32 : 16, G = A->cache.n_heads;
+  const int64_t rows = (int64_t)A->n_nodes * (A->n_heads / G), row_tiles = (rows + 15) / 16;
+  const int most = A->cache.head_dim <= 128 ? 8 : 4;
+  P.groups = (int)((row_tiles + most - 1) / most);
+  P.tile_rows = (int)((row_tiles + P.groups - 1) / P.groups);
+  P.pos_waves = P.tile_rows == 1 ? 4 : P.tile_rows == 2 ? 2 : 1;
+  P.cache_tiles = (int)(((int64_t)A->n_cache + AT - 1) / AT);
+  P.tree_tiles = (A->n_nodes + AT - 1) / AT;
+  P.gap = P.cache_tiles;
+  // R-SWA: no node sees what lies between the reference positions and the first root's window
+  if (A->window > 0 && !A->scores && A->n_cache >= A->prefill_len) {
+    const int64_t lo = (int64_t)A->n_cache + 1 - A->window;
+    const int from = (int)(((int64_t)A->prefill_len + AT - 1) / AT), to = lo > 0 ? (int)(lo / AT) : 0;
+    if (to > from) {
+      P.gap = from;
+      P.skip = to - from;
+    }
+  }
+  const int64_t tiles = (int64_t)P.cache_tiles - P.skip + P.tree_tiles;
+  const int64_t want = 2048 / ((int64_t)G * P.groups * P.tile_rows * P.pos_waves);
+  int64_t splits = (tiles + P.pos_waves - 1) / P.pos_waves;
+  if (splits > want) splits = want;
+  if (splits > 1024) splits = 1024;
+  if (splits < 1) splits = 1;
+  const int64_t per = (tiles + splits - 1) / splits;
+  P.splits = (int)((tiles + per - 1) / per);
+  return P;
+}
+
+// Floats of workspace for the splits' sums.
+size_t dsh_tree_attention_work(const dsh_tree_attn_t *A) {
+  const attend_plan P = attend_cut(A);
+  if (P.splits == 1) return 0;
+  return (size_t)A->cache.n_heads * P.groups * P.splits * 16 * P.tile_rows * (A->cache.head_dim + 2);
+}
+
+hipError_t dsh_launch_tree_attention(const dsh_tree_attn_t *A, float *work, hipStream_t s) {
   if (A->n_nodes < 1 || A->n_nodes > DSH_TREE_MAX) return hipErrorInvalidValue;
-  const dim3 g(A->n_nodes, A->n_heads);
-#define CASE(D, BF)                         \
-  case D:                                   \
-    k_tree_attend<D, BF><<<g, 256, 0, s>>>(*A); \
+  attend_plan P = attend_cut(A);
+  const int D = A->cache.head_dim, W = P.tile_rows * P.pos_waves;
+  if (W > 8 || P.groups > 65535 || (P.splits > 1 && !work)) return hipErrorInvalidValue;
+  P.part = work;
+  P.ml = work ? work + (size_t)A->cache.n_heads * P.groups * P.splits * 16 * P.tile_rows * D : nullptr;
+  const dim3 grid(P.splits, A->cache.n_heads, P.groups);
+  const size_t lds = (size_t)(P.pos_waves - 1) * P.tile_rows * 16 * D * 4;
+#define CASE(D, BF)                                                                   \
+  case D:                                                                             \
+    if (W <= 4)                                                                       \
+      k_tree_attend<D, BF, 4><<<grid, 64 * W, lds, s>>>(*A, P);                       \
+    else                                                                              \
+      k_tree_attend<D, BF, 8><<<grid, 64 * W, lds, s>>>(*A, P);                       \
+    if (P.splits > 1)                                                                 \
+      k_tree_join<D><<<dim3(A->n_nodes * (A->n_heads / A->cache.n_heads), A->cache.n_heads), 256, 0, s>>>(*A, P); \
     break;
   if (A->cache.bf16) {
-    BY_DIM(A->cache.head_dim, true, CASE)
+    BY_DIM(D, true, CASE)
   } else {
-    BY_DIM(A->cache.head_dim, false, CASE)
+    BY_DIM(D, false, CASE)
   }
 #undef CASE
   return hipGetLastError();

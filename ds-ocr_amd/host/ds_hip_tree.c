@@ -122,7 +122,12 @@ int ds_hip_tree_attention(float *out_dev, int64_t out_stride, float *lse_dev, fl
   a.scale = scale;
   int dev;
   if (enter(&dev)) return -1;
-  return leave(dev, me, dsh_launch_tree_attention(&a, dsr_stream));
+  float *work = (float *)dsr_scratch(DSR_SLOT_TREE, dsh_tree_attention_work(&a) * sizeof(float));
+  if (!work) {
+    leave(dev, me, hipSuccess);
+    return -1;
+  }
+  return leave(dev, me, dsh_launch_tree_attention(&a, work, dsr_stream));
 }
 
 static int verify(const char *me, int *path_dev, int *result_dev, const float *p, int64_t p_stride, const float *q,
