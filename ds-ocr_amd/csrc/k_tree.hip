@@ -12,17 +12,18 @@ typedef unsigned long long u64;
 // ---------------------------------------------------------------------------- the tree
 // Every node's ancestors-or-self as 128 bits and its depth, from the parents, by pointer doubling: after round r a node
 // knows its next 2^r ancestors, so that a chain of 128 takes 7 rounds. A padding node (a parent outside [-1, i), or a padding
-// node above it) has no bits. Called by every thread of a block of at least DSH_TREE_MAX.
+// node above it) has no bits. Called by every thread of a block of at least DSH_TREE_MAX with its node's parent.
 struct tree_lds {
   u64 anc[DSH_TREE_MAX][2];
   int up[DSH_TREE_MAX];
 };
-__device__ void tree_ancestors(tree_lds &t, const int *parents, int n) {
+__device__ __forceinline__ int tree_parent(const int *parents, int n) {
+  return (int)threadIdx.x < n ? parents[threadIdx.x] : -2;
+}
+__device__ void tree_ancestors(tree_lds &t, int up, int n) {
   const int i = threadIdx.x;
   u64 lo = 0, hi = 0;
-  int up = -2;
   if (i < n) {
-    up = parents[i];
     if (up < -1 || up >= i) up = -2;
     lo = i < 64 ? 1ull << i : 0;
     hi = i < 64 ? 0 : 1ull << (i - 64);
@@ -71,8 +72,7 @@ __device__ __forceinline__ bool tree_in_window(int p, int pos, int prefill_len, 
 #define ATT_SLACK 10.0f
 #define ATT_L2E 1.44269504088896340736f
 
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // How a launch cuts the work; a tile is AT positions of the cache (tiles in [gap, gap + skip) are seen by no node and left out)
@@ -80,7 +80,9 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 struct attend_plan {
   int tile_rows, pos_waves;  // 16-row tiles and shares of the positions in a block: a wave each
   int groups, splits;        // blocks per key head: groups of tile_rows tiles of rows, splits of the tiles of positions
-  int cache_tiles, tree_tiles, gap, skip;
+  int cache_tiles, tree_tiles, gap, skip, per;  // per: tiles of a split
+  int grp;                                       // query heads per key head
+  float inv_nodes;                               // 1 / n_nodes
   float *part, *ml;          // [head][group][split][16 * tile_rows] x D, and the maximum and sum
 };
 
@@ -256,28 +258,51 @@ struct frag_bf16 {
 // A block: tile_rows x pos_waves waves over one split of the tiles of one key head; the waves of a row tile put their sums
 // together, and the block writes them for k_tree_join (splits > 1) or finishes its rows itself.
 template <int D, bool BF, int W>
-__global__ void __launch_bounds__(64 * W) k_tree_attend(dsh_tree_attn_t A, attend_plan P) {
+__global__ void __launch_bounds__(64 * W, W == 4 && D <= 128 ? 2 : 1) k_tree_attend(dsh_tree_attn_t A, attend_plan P) {
   typedef typename std::conditional<BF, frag_bf16<D>, frag_f32<D>>::type frag;
   constexpr int AT = frag::AT, NV = AT / 4;  // scores a lane
   __shared__ tree_lds t;
-  __shared__ float s_m[W][16], s_l[W][16];
-  extern __shared__ __attribute__((aligned(16))) float s_o[];  // [pos_waves - 1][tile_rows][16][D]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const int G = A.cache.n_heads, grp = A.n_heads / G, T = A.n_nodes, R = T * grp;
+  __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ bool s_live[32];
+  extern __shared__ __attribute__((aligned(16))) float s_o[];  // pos_waves > 1: [wave][16][min(D, 128) + 4]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+  const int T = A.n_nodes, R = T * P.grp;
   const int kh = blockIdx.y, z = blockIdx.z, split = blockIdx.x;
-  const int rt = wave % P.tile_rows, pw = wave / P.tile_rows;
+  const int pw = P.pos_waves == 4 ? wave : P.pos_waves == 2 ? wave >> 1 : 0, rt = wave - pw * P.tile_rows;
   const int row = 16 * (z * P.tile_rows + rt) + i;  // the lane's
-  const int rr = min(row, R - 1), node = rr % T, head = kh * grp + rr / T;
-  const int tiles = P.cache_tiles - P.skip + P.tree_tiles;
-  const int per = (tiles + P.splits - 1) / P.splits, t0 = split * per, t1 = min(t0 + per, tiles);
-  frag F;
-  F.load_q(A.q + node * A.q_stride + (int64_t)head * D, g);
+  const int rr = min(row, R - 1), rh = (int)(((float)rr + 0.5f) * P.inv_nodes);  // 2^17 rows at most: exact
+  const int node = rr - rh * T, head = kh * P.grp + rh;
+  const int tiles = P.cache_tiles - P.skip + P.tree_tiles, t0 = split * P.per, t1 = min(t0 + P.per, tiles);
   // what only the tree's own tiles, a window, scores and whole rows need
   const bool need = P.splits == 1 || A.scores || A.window > 0 || t1 > P.cache_tiles - P.skip;
-  if (need) tree_ancestors(t, A.parents, T);
+  const int parent = need ? tree_parent(A.parents, T) : -2;
+  frag F;
+  // a tile: its rows (the cache's or the tree's own) and how many there are; loads past them repeat the last one
+  struct where {
+    const void *k, *v;
+    int64_t rs;
+    int p0, end;
+    bool own;
+    __device__ __forceinline__ int64_t operator()(int x) const { return min(p0 + x, end - 1) * rs; }
+  };
+  const auto locate = [&](int tile) {
+    const int x = tile >= P.gap ? tile + P.skip : tile;
+    const bool own = x >= P.cache_tiles;
+    const dsh_kv_t &c = own ? A.tree : A.cache;
+    const int64_t h = kh * c.head_stride * (BF ? 2 : 4);
+    return where{(const char *)c.k + h, (const char *)c.v + h, c.row_stride, AT * (own ? x - P.cache_tiles : x),
+                 own ? T : A.n_cache, own};
+  };
+  where nx = locate(min(t0 + pw, tiles - 1));
+  F.load_q(A.q + node * A.q_stride + (int64_t)head * D, g);
+  F.load_k(nx.k, nx, i, g);
+  F.load_v(nx.v, nx, i, g);
+  if (need) tree_ancestors(t, parent, T);
   const u64 anc0 = need ? t.anc[node][0] : 0, anc1 = need ? t.anc[node][1] : 0;
   const bool live = !need || (anc0 | anc1);
+  // the lane's row sees the positions below prefill_len and from lo on (all of them without a window)
   const int pos = A.n_cache + __popcll(anc0) + __popcll(anc1) - 1;
+  const int lo = A.window > 0 && pos >= A.prefill_len ? max(A.prefill_len, pos + 1 - A.window) : 0;
   const float inf = __builtin_huge_valf();
   float m = -inf, l = 0.0f, ml2 = 0.0f;
   f32x4 o[D / 16];
@@ -285,32 +310,32 @@ __global__ void __launch_bounds__(64 * W) k_tree_attend(dsh_tree_attn_t A, atten
   for (int b = 0; b < D / 16; b++) o[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float *sc = A.scores ? A.scores + ((int64_t)head * T + node) * A.score_stride : nullptr;
 
+  const int lo_most = A.n_cache + T - A.window;  // from here on every node's window holds a row
   for (int tile = t0 + pw; tile < t1; tile += P.pos_waves) {
-    int x = tile >= P.gap ? tile + P.skip : tile;
-    const bool own = x >= P.cache_tiles;
-    const dsh_kv_t &c = own ? A.tree : A.cache;
-    const int p0 = AT * (own ? x - P.cache_tiles : x), end = own ? T : A.n_cache;
-    const auto at = [&](int k) { return (int64_t)min(p0 + k, end - 1) * c.row_stride + kh * c.head_stride; };
-    F.load_k(c.k, at, i, g);
-    F.load_v(c.v, at, i, g);
+    const bool own = nx.own;
+    const int p0 = nx.p0, end = nx.end;
     float s[NV];
     F.scores(s);
+    // the next tile's K while this one's V is on its way, then its V; without a branch (past the end the last tile
+    // again), so that the waits are counted and neither waits for the other
+    nx = locate(min(tile + P.pos_waves, tiles - 1));
+    F.load_k(nx.k, nx, i, g);
 #pragma unroll
     for (int k = 0; k < NV; k++) s[k] *= A.scale;
-    bool part = !live || p0 + AT > end || own || A.window > 0;
-    if (__any(part)) {  // some position is not seen by some row
+    if (own || p0 + AT > end || (A.window > 0 && p0 + AT > A.prefill_len && p0 < lo_most)) {
+      // some position is not seen by some row
       uint32_t seen = 0;
 #pragma unroll
       for (int k = 0; k < NV; k++) {
         const int j = p0 + 16 * (k >> 2) + 4 * g + (k & 3);
         bool see = live && j < end;
+        int p = j;
         if (own) {
           const int a = min(j, DSH_TREE_MAX - 1);
           see = see && (((a < 64 ? anc0 >> a : anc1 >> (a - 64)) & 1) != 0);
-          if (A.window > 0 && see) see = tree_in_window(A.n_cache + tree_depth(t.anc[a]), pos, A.prefill_len, A.window);
-        } else {
-          see = see && tree_in_window(j, pos, A.prefill_len, A.window);
+          if (A.window > 0) p = A.n_cache + tree_depth(t.anc[a]);
         }
+        see = see && (p < A.prefill_len || p >= lo);
         s[k] = see ? s[k] : -inf;
         seen |= (uint32_t)see << k;
       }
@@ -334,7 +359,7 @@ __global__ void __launch_bounds__(64 * W) k_tree_attend(dsh_tree_attn_t A, atten
 #pragma unroll
       for (int k = 0; k < NV; k++) {
         const int j = p0 + 16 * (k >> 2) + 4 * g + (k & 3);
-        if (j < end) sc[own ? (int64_t)A.n_cache + j : j] = s[k];
+        if (j < end) sc[own ? (int64_t)A.n_cache + j : j] = live ? s[k] : -inf;
       }
     }
     float mx = s[0];
@@ -357,73 +382,68 @@ __global__ void __launch_bounds__(64 * W) k_tree_attend(dsh_tree_attn_t A, atten
       l += s[k];
     }
     F.add(s, o);
+    F.load_v(nx.v, nx, i, g);
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
 
-  if (P.pos_waves > 1) {
-    if (g == 0) {
-      s_m[wave][i] = m;
-      s_l[wave][i] = l;
+  // A row's sums, for the join or finished: factor * (what the waves of its tile have).
+  const auto put = [&](int node, int head, int64_t at, int d, f32x4 y, float m, float l, bool live) {
+    if (P.splits > 1) {
+      *(f32x4 *)(P.part + at * D + d) = y;
+      if (d == 0) *(f32x2 *)(P.ml + 2 * at) = f32x2{m, l};
+      return;
     }
+    const bool none = !live || l == 0.0f;
+    y = none ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : y * (1.0f / l);
+    *(f32x4 *)(A.out + node * A.out_stride + (int64_t)head * D + d) = y;
+    if (A.lse && d == 0) A.lse[(int64_t)head * T + node] = none ? -inf : m + logf(l);
+  };
+  const int64_t at0 = (((int64_t)kh * P.groups + z) * P.splits + split) * 16 * P.tile_rows;
+  if (P.pos_waves == 1) {
+    if (row >= R) return;
+#pragma unroll
+    for (int b = 0; b < D / 64; b++)
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        put(node, head, at0 + 16 * rt + i, frag::dim(b, r, g), f32x4{o[4 * b][r], o[4 * b + 1][r], o[4 * b + 2][r], o[4 * b + 3][r]},
+            m, l, live);
+    return;
+  }
+  // the waves of a row tile: every thread of the block adds up pieces of four dimensions
+  if (g == 0) {
+    s_m[wave][i] = m;
+    s_l[wave][i] = l;
+    s_live[16 * rt + i] = live;
+  }
+  constexpr int CH = D < 128 ? D : 128;  // dimensions at a time, for the LDS
+#pragma unroll
+  for (int c = 0; c < D; c += CH) {
+    const int width = min(CH, D - c);
+    if (c) __syncthreads();
+#pragma unroll
+    for (int b = c / 64; b < (c + CH) / 64 && b < D / 64; b++)
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        *(f32x4 *)(s_o + (wave * 16 + i) * (CH + 4) + frag::dim(b, r, g) - c) =
+            f32x4{o[4 * b][r], o[4 * b + 1][r], o[4 * b + 2][r], o[4 * b + 3][r]};
     __syncthreads();
-    float M = -inf;
-    for (int w = 0; w < P.pos_waves; w++) M = fmaxf(M, s_m[w * P.tile_rows + rt][i]);
-    l = 0.0f;
-    for (int w = 0; w < P.pos_waves; w++) {
-      const float mw = s_m[w * P.tile_rows + rt][i];
-      l += s_l[w * P.tile_rows + rt][i] * (mw == M ? 1.0f : att_exp(mw - M));
-    }
-    const float f = m == M ? 1.0f : att_exp(m - M);
-    m = M;
-#pragma unroll
-    for (int b = 0; b < D / 16; b++) o[b] *= f;
-    if (pw > 0) {
-      float *d = s_o + (((pw - 1) * P.tile_rows + rt) * 16 + i) * D;
-#pragma unroll
-      for (int b = 0; b < D / 64; b++)
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-          *(f32x4 *)(d + frag::dim(b, r, g)) = f32x4{o[4 * b][r], o[4 * b + 1][r], o[4 * b + 2][r], o[4 * b + 3][r]};
-    }
-    __syncthreads();
-    if (pw > 0) return;
-    for (int w = 0; w < P.pos_waves - 1; w++) {
-      const float *d = s_o + ((w * P.tile_rows + rt) * 16 + i) * D;
-#pragma unroll
-      for (int b = 0; b < D / 64; b++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const f32x4 y = *(const f32x4 *)(d + frag::dim(b, r, g));
-#pragma unroll
-          for (int e = 0; e < 4; e++) o[4 * b + e][r] += y[e];
-        }
+    for (int x = threadIdx.x; x < 16 * P.tile_rows * (width / 4); x += 256) {
+      const int r = x / (width / 4), d = 4 * (x - r * (width / 4)), r16 = r & 15, tile = r >> 4, row = 16 * z * P.tile_rows + r;
+      if (row >= R) continue;
+      float M = -inf, L = 0.0f;
+      for (int w = 0; w < P.pos_waves; w++) M = fmaxf(M, s_m[w * P.tile_rows + tile][r16]);
+      f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int w = 0; w < P.pos_waves; w++) {
+        const int v = w * P.tile_rows + tile;
+        const float mw = s_m[v][r16], f = mw == M ? 1.0f : att_exp(mw - M);
+        L += s_l[v][r16] * f;
+        y += *(const f32x4 *)(s_o + (v * 16 + r16) * (CH + 4) + d) * f;
+      }
+      const int h = (int)(((float)row + 0.5f) * P.inv_nodes), nd = row - h * T;
+      put(nd, kh * P.grp + h, at0 + r, c + d, y, M, L, s_live[r]);
     }
   }
-  if (row >= R) return;
-  float *to;
-  float f = 1.0f;
-  if (P.splits == 1) {
-    to = A.out + node * A.out_stride + (int64_t)head * D;
-    f = !live || l == 0.0f ? 0.0f : 1.0f / l;
-    if (A.lse && g == 0) A.lse[(int64_t)head * T + node] = f == 0.0f ? -inf : m + logf(l);
-  } else {
-    const int64_t at = (((int64_t)kh * P.groups + z) * P.splits + split) * 16 * P.tile_rows + 16 * rt + i;
-    to = P.part + at * D;
-    if (g == 0) {
-      P.ml[2 * at] = m;
-      P.ml[2 * at + 1] = l;
-    }
-  }
-  const bool zero = P.splits == 1 && (!live || l == 0.0f);
-#pragma unroll
-  for (int b = 0; b < D / 64; b++)
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      f32x4 y = f32x4{o[4 * b][r], o[4 * b + 1][r], o[4 * b + 2][r], o[4 * b + 3][r]} * f;
-      if (zero) y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      *(f32x4 *)(to + frag::dim(b, r, g)) = y;
-    }
 }
 
 // The splits of one row put together, in their order: a block of D threads per row, the maxima and sums by its first wave.
@@ -431,11 +451,11 @@ template <int D>
 __global__ void __launch_bounds__(256) k_tree_join(dsh_tree_attn_t A, attend_plan P) {
   __shared__ tree_lds t;
   __shared__ float s_f[1024], s_inv;
-  const int G = A.cache.n_heads, grp = A.n_heads / G, T = A.n_nodes;
-  const int row = blockIdx.x, kh = blockIdx.y, node = row % T, head = kh * grp + row / T;
-  const int z = row / (16 * P.tile_rows), in = row - z * 16 * P.tile_rows, stride = 16 * P.tile_rows;
+  const int T = A.n_nodes, row = blockIdx.x, kh = blockIdx.y, rh = (int)(((float)row + 0.5f) * P.inv_nodes);
+  const int node = row - rh * T, head = kh * P.grp + rh;
+  const int z = (row >> 4) / P.tile_rows, in = row - z * 16 * P.tile_rows, stride = 16 * P.tile_rows;
   const int64_t at = ((int64_t)kh * P.groups + z) * P.splits * stride + in;
-  tree_ancestors(t, A.parents, T);
+  tree_ancestors(t, tree_parent(A.parents, T), T);
   const bool live = t.anc[node][0] | t.anc[node][1];
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
@@ -685,13 +705,18 @@ static attend_plan attend_cut(const dsh_tree_attn_t *A) {
     }
   }
   const int64_t tiles = (int64_t)P.cache_tiles - P.skip + P.tree_tiles;
-  const int64_t want = 2048 / ((int64_t)G * P.groups * P.tile_rows * P.pos_waves);
+  // two blocks of four waves fit a CU, one of more
+  const int64_t want = (P.tile_rows * P.pos_waves <= 4 ? 512 : 256) / ((int64_t)G * P.groups);
+  // up to four tiles a wave cost less than a second kernel that joins splits
   int64_t splits = (tiles + P.pos_waves - 1) / P.pos_waves;
+  if (splits <= 4) splits = 1;
   if (splits > want) splits = want;
   if (splits > 1024) splits = 1024;
   if (splits < 1) splits = 1;
-  const int64_t per = (tiles + splits - 1) / splits;
-  P.splits = (int)((tiles + per - 1) / per);
+  P.per = (int)((tiles + splits - 1) / splits);
+  P.splits = (int)((tiles + P.per - 1) / P.per);
+  P.grp = A->n_heads / G;
+  P.inv_nodes = 1.0f / (float)A->n_nodes;
   return P;
 }
 
@@ -710,7 +735,7 @@ hipError_t dsh_launch_tree_attention(const dsh_tree_attn_t *A, float *work, hipS
   P.part = work;
   P.ml = work ? work + (size_t)A->cache.n_heads * P.groups * P.splits * 16 * P.tile_rows * D : nullptr;
   const dim3 grid(P.splits, A->cache.n_heads, P.groups);
-  const size_t lds = (size_t)(P.pos_waves - 1) * P.tile_rows * 16 * D * 4;
+  const size_t lds = P.pos_waves > 1 ? (size_t)W * 16 * ((D < 128 ? D : 128) + 4) * 4 : 0;
 #define CASE(D, BF)                                                                   \
   case D:                                                                             \
     if (W <= 4)                                                                       \
