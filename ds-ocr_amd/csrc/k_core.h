@@ -383,10 +383,14 @@ typedef struct {
 } dsh_tree_attn_t;
 size_t dsh_tree_attention_work(const dsh_tree_attn_t *A); /* floats */
 hipError_t dsh_launch_tree_attention(const dsh_tree_attn_t *A, float *work, hipStream_t s);
-/* target: greedy (p, q, u unused); else p, optionally q, and u. */
+/* words: DSH_VERIFY_WORDS 64-bit words, zeroed when they are allocated; epoch differs from every earlier launch's on them.
+ * *derr is set (system scope) when a block's wait for the others' sums gives up: the answer is then an empty path and -1. */
+#define DSH_VERIFY_WORDS ((DSH_TREE_MAX + 4) * 128)
 hipError_t dsh_launch_tree_verify(int *path, int *result, const float *p, int64_t p_stride, const float *q,
-                                  int64_t q_stride, int vocab, const int *target, const int *tokens, const int *parents,
-                                  int n_nodes, const float *u, hipStream_t s);
+                                  int64_t q_stride, int vocab, const int *tokens, const int *parents, int n_nodes,
+                                  const float *u, unsigned long long *words, unsigned epoch, int *derr, hipStream_t s);
+hipError_t dsh_launch_tree_verify_greedy(int *path, int *result, const int *target, const int *tokens, const int *parents,
+                                         int n_nodes, hipStream_t s);
 typedef struct {
   dsh_kv_t cache, tree;
   const int *path, *result;

@@ -1,9 +1,12 @@
-// k_evict.hip — which rows of a KV cache stay (k_kv_evict: per head the rows with the least attention weight go), and the
-// moves that bring them together.
+// k_evict.hip — which rows of a KV cache stay (k_kv_select: per head the rows with the least attention weight go), and the
+// moves that bring them together (k_kv_move).
 #include "dsh.h"
 #include "k_core.h"
 
 #define ET 1024
+#define EW (ET / 64)
+
+typedef unsigned long long u64;
 
 // Floats in ascending order as unsigned numbers; -0 as 0, a NaN as -inf.
 __device__ __forceinline__ uint32_t evict_key(float a) {
@@ -12,81 +15,214 @@ __device__ __forceinline__ uint32_t evict_key(float a) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exclusive prefix sum of v over the block's threads; *total receives the sum.
-__device__ int evict_scan(int v, int *s_w, int *total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int a = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int b = __shfl_up(a, o);
-    if (lane >= o) a += b;
-  }
-  __syncthreads();
-  if (lane == 63) s_w[wave] = a;
-  __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < ET / 64; w++) {
-    before += w < wave ? s_w[w] : 0;
-    all += s_w[w];
-  }
-  *total = all;
-  return before + a - v;
+// A row of a head as a number: `gone` = n - keep rows with the lowest numbers go, the lower row first among equal ones. Where
+// there are unguarded rows enough, a guarded row is above all; where not, an unguarded one is below all.
+__device__ __forceinline__ uint32_t evict_number(float a, bool guarded, bool spill) {
+  return guarded == spill ? evict_key(a) : spill ? 0u : 0xFFFFFFFFu;
 }
 
-// One block per head: the threshold by radix select over 8-bit digits, then the rows that go, the holes they leave below
-// `keep` and the rows that fill them.
-template <int D, typename T>
-__global__ void __launch_bounds__(ET) k_kv_evict(dsh_kv_evict_t A) {
-  __shared__ int s_hist[256], s_w[ET / 64], s_digit, s_left;
+// Three counts of a wave (the same in all its lanes) summed over the block.
+__device__ __forceinline__ void evict_sums(int (*s_cnt)[EW], int &a, int &b, int &c) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __syncthreads();
+  if (lane < 3) s_cnt[lane][wave] = lane == 0 ? a : lane == 1 ? b : c;
+  __syncthreads();
+  int x = lane < 48 ? s_cnt[lane >> 4][lane & 15] : 0;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o);
+  a = __builtin_amdgcn_readlane(x, 0);
+  b = __builtin_amdgcn_readlane(x, 16);
+  c = __builtin_amdgcn_readlane(x, 32);
+}
+
+// The gone-th lowest number T, two bits at a step: each counts the numbers below three candidates by wave votes (count(t)
+// is a wave's), which costs the same whatever the numbers are; a histogram in LDS piles up on the few exponents that weights
+// have. left: how many of those equal to T go.
+template <typename F>
+__device__ __forceinline__ void evict_threshold(int (*s_cnt)[EW], int gone, uint32_t &T, int &left, F count) {
+  T = 0;
+  left = gone;
+  if (gone == 0) return;
+  for (int shift = 30; shift >= 0; shift -= 2) {
+    const uint32_t t1 = T | 1u << shift, t2 = T | 2u << shift, t3 = T | 3u << shift;
+    int c1 = 0, c2 = 0, c3 = 0;
+    count(t1, t2, t3, c1, c2, c3);
+    evict_sums(s_cnt, c1, c2, c3);
+    const int c = c3 < gone ? c3 : c2 < gone ? c2 : c1;
+    if (c < gone) {
+      T = c3 < gone ? t3 : c2 < gone ? t2 : t1;
+      left = gone - c;
+    }
+  }
+}
+
+// Exclusive prefix of N cells (a multiple of 64) by one wave; s[N] becomes the sum.
+template <int N>
+__device__ __forceinline__ void evict_prefix(int *s) {
+  constexpr int P = N / 64;
+  const int lane = threadIdx.x & 63;
+  int v[P], sum = 0;
+#pragma unroll
+  for (int k = 0; k < P; k++) {
+    v[k] = s[P * lane + k];
+    sum += v[k];
+  }
+  int x = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 63) s[N] = x;
+  x -= sum;
+#pragma unroll
+  for (int k = 0; k < P; k++) {
+    s[P * lane + k] = x;
+    x += v[k];
+  }
+}
+
+// One block per head, up to 1024 E rows in registers; thread t has the rows 1024 e + t. Ranks (among the equal numbers, then of
+// the holes below `keep` and of the rows that fill them) come from votes too: a count for every 64 rows, a prefix over those.
+// Workspace: per head a count, then holes [most] and movers [most], most = min(n - keep, keep).
+template <int E>
+__global__ void __launch_bounds__(ET) k_kv_select(dsh_kv_evict_t A, int most) {
+  constexpr int N = E * EW;
+  __shared__ int s_cnt[3][EW], s_a[N + 1], s_b[N + 1];
+  extern __shared__ uint16_t s_mv[];  // [most]
+  const int h = blockIdx.x, n = A.n, keep = A.keep, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const float *acc = A.acc + h * A.acc_stride;
+  const int *pos = A.pos ? A.pos + h * A.pos_stride : nullptr;
+  int *count = A.work + h, *hole = A.work + A.cache.n_heads + (int64_t)h * 2 * most, *mover = hole + most;
+  const u64 below = (1ull << lane) - 1;
+  uint32_t key[E];
+  int p[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int j = ET * e + tid;
+    key[e] = __float_as_uint(j < n ? acc[j] : 0.0f);
+    p[e] = j < n && pos ? pos[j] : j;
+  }
+  uint32_t guard = 0;
+  int free_rows = 0, none = 0, none2 = 0;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const bool g = p[e] < A.sink || p[e] >= A.recent_from;
+    guard |= (uint32_t)g << e;
+    free_rows += __popcll(__ballot(ET * e + tid < n && !g));
+  }
+  evict_sums(s_cnt, free_rows, none, none2);
+  const int gone = n - keep;
+  const bool spill = gone > free_rows;
+#pragma unroll
+  for (int e = 0; e < E; e++)
+    key[e] = ET * e + tid < n ? evict_number(__uint_as_float(key[e]), (guard >> e) & 1, spill) : 0xFFFFFFFFu;
+  uint32_t T;
+  int left;
+  evict_threshold(s_cnt, gone, T, left, [&](uint32_t t1, uint32_t t2, uint32_t t3, int &c1, int &c2, int &c3) {
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      c1 += __popcll(__ballot(key[e] < t1));
+      c2 += __popcll(__ballot(key[e] < t2));
+      c3 += __popcll(__ballot(key[e] < t3));
+    }
+  });
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int c = __popcll(__ballot(key[e] == T));
+    if (lane == 0) s_a[e * EW + wave] = c;
+  }
+  __syncthreads();
+  if (wave == 0) evict_prefix<N>(s_a);
+  __syncthreads();
+  uint32_t stays = 0;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int rank = s_a[e * EW + wave] + __popcll(__ballot(key[e] == T) & below);
+    stays |= (uint32_t)(ET * e + tid < n && (key[e] > T || (key[e] == T && rank >= left))) << e;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int j = ET * e + tid;
+    const bool s = (stays >> e) & 1;
+    const int ch = __popcll(__ballot(j < keep && !s)), cm = __popcll(__ballot(j >= keep && s));
+    if (lane == 0) {
+      s_a[e * EW + wave] = ch;
+      s_b[e * EW + wave] = cm;
+    }
+  }
+  __syncthreads();
+  if (wave == 0) evict_prefix<N>(s_a);
+  if (wave == 1) evict_prefix<N>(s_b);
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int j = ET * e + tid;
+    const bool m = j >= keep && ((stays >> e) & 1);
+    const int r = s_b[e * EW + wave] + __popcll(__ballot(m) & below);
+    if (m) {
+      s_mv[r] = (uint16_t)j;
+      mover[r] = j;
+    }
+  }
+  if (tid == 0) *count = s_a[N];
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int j = ET * e + tid;
+    const bool o = j < keep && !((stays >> e) & 1);
+    const int r = s_a[e * EW + wave] + __popcll(__ballot(o) & below);
+    if (o) hole[r] = j;
+    if (j < keep) {
+      const int from = o ? s_mv[r] : j;
+      if (A.slots) A.slots[(int64_t)h * keep + j] = from;
+      if (A.acc_out) A.acc_out[h * A.acc_out_stride + j] = acc[from];
+      if (A.pos_out) A.pos_out[h * A.pos_out_stride + j] = pos[from];
+    }
+  }
+}
+
+// The same for more rows than that, read again at every step; a thread's rows are consecutive where ranks are counted.
+__global__ void __launch_bounds__(ET) k_kv_select_long(dsh_kv_evict_t A, int most) {
+  __shared__ int s_cnt[3][EW], s_a[ET + 1], s_b[ET + 1];
   const int h = blockIdx.x, n = A.n, keep = A.keep, tid = threadIdx.x;
   const float *acc = A.acc + h * A.acc_stride;
   const int *pos = A.pos ? A.pos + h * A.pos_stride : nullptr;
-  auto guarded = [&](int j) {
+  int *count = A.work + h, *hole = A.work + A.cache.n_heads + (int64_t)h * 2 * most, *mover = hole + most;
+  const auto guarded = [&](int j) {
     const int p = pos ? pos[j] : j;
     return p < A.sink || p >= A.recent_from;
   };
-  int v = 0, total;
-  for (int j = tid; j < n; j += ET) v += !guarded(j);
-  evict_scan(v, s_w, &total);
-  int gone = n - keep;               // rows that go
-  const bool all_free = gone > total;  // every unguarded row, and some of the guarded
-  if (all_free) gone -= total;
-  // among the rows of the class (guarded == all_free) the `gone` lowest go: the gone-th key, digit by digit
-  uint32_t prefix = 0;
-  int left = gone;  // how many of those with the prefix so far
-  for (int shift = 24; shift >= 0 && gone > 0; shift -= 8) {
-    __syncthreads();
-    if (tid < 256) s_hist[tid] = 0;
-    __syncthreads();
-    for (int j = tid; j < n; j += ET) {
-      const uint32_t k = evict_key(acc[j]);
-      if (guarded(j) == all_free && (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))))
-        atomicAdd(&s_hist[(k >> shift) & 255], 1);
+  int free_rows = 0, none = 0, none2 = 0;
+  for (int j0 = 0; j0 < n; j0 += ET) free_rows += __popcll(__ballot(j0 + tid < n && !guarded(min(j0 + tid, n - 1))));
+  evict_sums(s_cnt, free_rows, none, none2);
+  const int gone = n - keep;
+  const bool spill = gone > free_rows;
+  const auto number = [&](int j) { return evict_number(acc[j], guarded(j), spill); };
+  uint32_t T;
+  int left;
+  evict_threshold(s_cnt, gone, T, left, [&](uint32_t t1, uint32_t t2, uint32_t t3, int &c1, int &c2, int &c3) {
+    for (int j0 = 0; j0 < n; j0 += ET) {
+      const uint32_t k = j0 + tid < n ? number(j0 + tid) : 0xFFFFFFFFu;
+      c1 += __popcll(__ballot(k < t1));
+      c2 += __popcll(__ballot(k < t2));
+      c3 += __popcll(__ballot(k < t3));
     }
-    __syncthreads();
-    int all;
-    const int c = tid < 256 ? s_hist[tid] : 0;
-    const int before = evict_scan(c, s_w, &all);
-    if (before < left && before + c >= left) {
-      s_digit = tid;
-      s_left = left - before;
-    }
-    __syncthreads();
-    prefix |= (uint32_t)s_digit << shift;
-    left = s_left;
-  }
-  // a thread's rows are consecutive: ranks in the order of the rows by one scan
-  const int per = (n + ET - 1) / ET, j0 = min(tid * per, n), j1 = min(j0 + per, n);
+  });
+  const int per = (int)(((int64_t)n + ET - 1) / ET);
+  const int j0 = (int)min((int64_t)tid * per, (int64_t)n), j1 = (int)min((int64_t)j0 + per, (int64_t)n);
   int ties = 0;
-  for (int j = j0; j < j1; j++) ties += gone > 0 && guarded(j) == all_free && evict_key(acc[j]) == prefix;
-  const int tie0 = evict_scan(ties, s_w, &total);
-  auto stays = [&](int j, int &tie) {
-    const bool g = guarded(j);
-    if (g != all_free) return g;  // guarded rows stay; unguarded ones go when the class is the guarded
-    if (gone == 0) return true;
-    const uint32_t k = evict_key(acc[j]);
-    if (k != prefix) return k > prefix;
-    return tie++ >= left;
+  for (int j = j0; j < j1; j++) ties += number(j) == T;
+  s_a[tid] = ties;
+  __syncthreads();
+  if (tid < 64) evict_prefix<ET>(s_a);
+  __syncthreads();
+  const int tie0 = s_a[tid];
+  const auto stays = [&](int j, int &tie) {
+    const uint32_t k = number(j);
+    return k > T || (k == T && tie++ >= left);
   };
   int holes = 0, movers = 0, tie = tie0;
   for (int j = j0; j < j1; j++) {
@@ -94,55 +230,101 @@ __global__ void __launch_bounds__(ET) k_kv_evict(dsh_kv_evict_t A) {
     holes += j < keep && !s;
     movers += j >= keep && s;
   }
-  int *mv = A.work + (int64_t)h * (n - keep), *slot = A.work + (int64_t)A.cache.n_heads * (n - keep) + (int64_t)h * keep;
-  int hole = evict_scan(holes, s_w, &total), mover = evict_scan(movers, s_w, &total);
-  tie = tie0;
-  for (int j = j0; j < j1; j++)
-    if (stays(j, tie) && j >= keep) mv[mover++] = j;
   __syncthreads();
-  tie = tie0;
-  for (int j = j0; j < min(j1, keep); j++) slot[j] = stays(j, tie) ? j : mv[hole++];
+  s_a[tid] = holes;
+  s_b[tid] = movers;
   __syncthreads();
-  float a = 0.0f;
+  if (tid < 64)
+    evict_prefix<ET>(s_a);
+  else if (tid < 128)
+    evict_prefix<ET>(s_b);
+  __syncthreads();
+  int oh = s_a[tid], om = s_b[tid];
+  tie = tie0;
+  for (int j = j0; j < j1; j++) {
+    const bool s = stays(j, tie);
+    if (j < keep && !s) hole[oh++] = j;
+    if (j >= keep && s) mover[om++] = j;
+  }
+  const int moves = s_a[ET];
+  if (tid == 0) *count = moves;
+  __syncthreads();
+  // the rows that stay where they are (all of them first), then the holes
   for (int j = tid; j < keep; j += ET) {
-    const int from = slot[j];
+    if (A.slots) A.slots[(int64_t)h * keep + j] = j;
+    if (A.acc_out && A.acc_out != A.acc) A.acc_out[h * A.acc_out_stride + j] = acc[j];
+    if (A.pos_out && A.pos_out != A.pos) A.pos_out[h * A.pos_out_stride + j] = pos[j];
+  }
+  __syncthreads();
+  for (int r = tid; r < moves; r += ET) {
+    const int j = hole[r], from = mover[r];
     if (A.slots) A.slots[(int64_t)h * keep + j] = from;
-    if (A.acc_out) {
-      a = acc[from];
-      A.acc_out[h * A.acc_out_stride + j] = a;
-    }
+    if (A.acc_out) A.acc_out[h * A.acc_out_stride + j] = acc[from];
     if (A.pos_out) A.pos_out[h * A.pos_out_stride + j] = pos[from];
   }
-  for (int j = tid >> 6; j < keep; j += ET / 64) {
-    const int from = slot[j];
-    if (from == j) continue;
-    const int64_t x = from * A.cache.row_stride + h * A.cache.head_stride, y = j * A.cache.row_stride + h * A.cache.head_stride;
-    for (int d = tid & 63; d < D; d += 64) {
-      ((T *)A.cache.k)[y + d] = ((const T *)A.cache.k)[x + d];
-      ((T *)A.cache.v)[y + d] = ((const T *)A.cache.v)[x + d];
+}
+
+// K and V rows of the movers into the holes, 16 bytes a thread, four pieces under way.
+template <int PIECES>  // 16-byte pieces of a row
+__global__ void __launch_bounds__(256) k_kv_move(dsh_kv_evict_t A, int most) {
+  const int h = blockIdx.y, count = A.work[h];
+  const int *hole = A.work + A.cache.n_heads + (int64_t)h * 2 * most, *mover = hole + most;
+  const int64_t rs = A.cache.row_stride * (A.cache.bf16 ? 2 : 4), hs = A.cache.head_stride * (A.cache.bf16 ? 2 : 4);
+  char *k = (char *)A.cache.k + h * hs, *v = (char *)A.cache.v + h * hs;
+  const int64_t total = (int64_t)count * 2 * PIECES, step = (int64_t)gridDim.x * 256;
+  for (int64_t x = blockIdx.x * 256 + threadIdx.x; x < total; x += 4 * step) {
+    u32x4 y[4];
+    char *to[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int64_t i = x + u * step;
+      to[u] = nullptr;
+      if (i < total) {
+        const int r = (int)(i / (2 * PIECES)), piece = (int)(i - (int64_t)r * 2 * PIECES);
+        char *b = piece < PIECES ? k + 16 * piece : v + 16 * (piece - PIECES);
+        to[u] = b + hole[r] * rs;
+        y[u] = *(const u32x4 *)(b + mover[r] * rs);
+      }
     }
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+      if (to[u]) *(u32x4 *)to[u] = y[u];
   }
 }
 
 extern "C" {
 
-// Per head the rows that move (n - keep at most) and the row of each slot.
-size_t dsh_kv_evict_work(int n_heads, int n, int keep) { return (size_t)n_heads * n; }
+static int evict_most(int n, int keep) { return n - keep < keep ? n - keep : keep; }
+
+size_t dsh_kv_evict_work(int n_heads, int n, int keep) { return (size_t)n_heads * (1 + 2 * (size_t)evict_most(n, keep)); }
 
 hipError_t dsh_launch_kv_evict(const dsh_kv_evict_t *A, hipStream_t s) {
-#define EV(D)                                                          \
-  case D:                                                              \
-    if (A->cache.bf16)                                                 \
-      k_kv_evict<D, uint16_t><<<A->cache.n_heads, ET, 0, s>>>(*A);     \
-    else                                                               \
-      k_kv_evict<D, float><<<A->cache.n_heads, ET, 0, s>>>(*A);        \
+  const int most = evict_most(A->n, A->keep), G = A->cache.n_heads;
+  const size_t lds = (size_t)(most + 1) * 2;  // 32 KB at most
+  if (A->n <= 4 * ET)
+    k_kv_select<4><<<G, ET, lds, s>>>(*A, most);
+  else if (A->n <= 8 * ET)
+    k_kv_select<8><<<G, ET, lds, s>>>(*A, most);
+  else if (A->n <= 16 * ET)
+    k_kv_select<16><<<G, ET, lds, s>>>(*A, most);
+  else if (A->n <= 32 * ET)
+    k_kv_select<32><<<G, ET, lds, s>>>(*A, most);
+  else
+    k_kv_select_long<<<G, ET, 0, s>>>(*A, most);
+  if (most == 0) return hipGetLastError();
+  const int pieces = A->cache.head_dim / (A->cache.bf16 ? 8 : 4);
+  const int64_t want = ((int64_t)most * 2 * pieces + 1023) / 1024, cap = G < 2048 ? 2048 / G : 1;
+  const dim3 g((unsigned)(want < cap ? want : cap), G);
+#define MV(N)                                      \
+  case N:                                          \
+    k_kv_move<N><<<g, 256, 0, s>>>(*A, most);      \
     break;
-  switch (A->cache.head_dim) {
-    EV(64) EV(128) EV(192) EV(256)
+  switch (pieces) {
+    MV(8) MV(16) MV(24) MV(32) MV(48) MV(64)
     default:
       return hipErrorInvalidValue;
   }
-#undef EV
+#undef MV
   return hipGetLastError();
 }
 

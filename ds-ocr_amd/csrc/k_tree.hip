@@ -484,150 +484,329 @@ __global__ void __launch_bounds__(256) k_tree_join(dsh_tree_attn_t A, attend_pla
 }
 
 // ---------------------------------------------------------------------------- verification
+// A step's answer hangs on a handful of probabilities and on one row of the vocabulary (one more for every draft that was
+// drawn from q and rejected), so what counts is the chain of dependent reads. Every block walks the tree by itself (a wave
+// holds a node a lane, twice, with the probabilities at its token fetched ahead), and owns 1/gridDim.x of the row: a sum over
+// the row is each block's share, told to all others through tagged words. The last such sum also says which block the drawn
+// token lies in, and that block finds it.
+
 // A probability: what is not positive and finite counts as 0.
 __device__ __forceinline__ double prob(float x) { return x > 0.0f && x < __builtin_huge_valf() ? (double)x : 0.0; }
-
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-  return v;
-}
 
 struct verify_args {
   int *path, *result;
   const float *p, *q, *u;
-  const int *target, *tokens, *parents;
+  const int *tokens, *parents;
   int64_t p_stride, q_stride;
-  int vocab, n;
+  int vocab, n, share;  // share: values of a block
+  u64 *words;           // [rounds][64][2]
+  unsigned epoch;
+  int *derr;
 };
 
-// What is left of a context's distribution: max(p - c q, 0), or p without the rejected tokens.
-struct residual {
-  const float *p, *q;
-  double c;
-  const int *gone;  // LDS
-  int n_gone;
-  __device__ __forceinline__ double at(int v) const {
-    const double x = prob(p[v]);
-    if (q) return fmax(x - c * prob(q[v]), 0.0);
-    for (int k = 0; k < n_gone; k++)
-      if (gone[k] == v) return 0.0;
-    return x;
-  }
-};
+#define VB 256  // threads; eight consecutive values each at a time
+#define VC (8 * VB)
+#define VERIFY_TICKS 400000000ull  // of the 100 MHz clock: four seconds
 
-#define VT 1024
-// Sum of the residual over [lo, hi) (every thread gets it).
-__device__ double residual_sum(const residual &r, int lo, int hi, double *s_w) {
-  double a = 0.0;
-  for (int v = lo + threadIdx.x; v < hi; v += VT) a += r.at(v);
-  a = wave_sum64(a);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s_w[threadIdx.x >> 6] = a;
-  __syncthreads();
-  a = 0.0;
-  for (int w = 0; w < VT / 64; w++) a += s_w[w];
-  return a;
+typedef float f32x4_dw __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ double read64(double v, int lane) {
+  const u64 x = (u64)__double_as_longlong(v);
+  const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)x, lane), hi = __builtin_amdgcn_readlane((int)(unsigned)(x >> 32), lane);
+  return __longlong_as_double((long long)((u64)hi << 32 | lo));
 }
 
-// One block: the walk (every thread the same), and the draw from what is left.
-__global__ void __launch_bounds__(VT) k_tree_verify(verify_args A) {
-  __shared__ int s_par[DSH_TREE_MAX], s_tok[DSH_TREE_MAX], s_gone[DSH_TREE_MAX];
-  __shared__ double s_w[VT / 64];
-  const int n = A.n, tid = threadIdx.x;
-  if (tid < n) {
-    s_par[tid] = A.parents[tid];
-    s_tok[tid] = A.tokens[tid];
-    A.path[tid] = -1;
+struct verify_lds {
+  double part[VB / 64], sum[64];
+  unsigned gone[VC / 32];
+  int found, last, fail;
+};
+
+// What is left of the thread's eight values from v on: max(p - c q, 0), or p without the rejected tokens (bits of gone).
+__device__ __forceinline__ void verify_left(double *w, const float *p, const float *q, double c, int v, int end, unsigned gone) {
+  float a[8], b[8];
+  if (v + 8 <= end) {
+    *(f32x4_dw *)a = *(const f32x4_dw *)(p + v);
+    *(f32x4_dw *)(a + 4) = *(const f32x4_dw *)(p + v + 4);
+    if (q) {
+      *(f32x4_dw *)b = *(const f32x4_dw *)(q + v);
+      *(f32x4_dw *)(b + 4) = *(const f32x4_dw *)(q + v + 4);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      a[e] = v + e < end ? p[v + e] : 0.0f;
+      b[e] = q && v + e < end ? q[v + e] : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    w[e] = prob(a[e]);
+    if (q)
+      w[e] = fmax(w[e] - c * prob(b[e]), 0.0);
+    else if ((gone >> e) & 1)
+      w[e] = 0.0;
+  }
+}
+
+// The rejected tokens among [v0, v0 + VC) as bits: the tokens of the lanes with rej.
+__device__ void verify_mark(verify_lds &L, int v0, int tok0, bool rej0, int tok1, bool rej1) {
+  __syncthreads();
+  if (threadIdx.x < VC / 32) L.gone[threadIdx.x] = 0;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const unsigned a = (unsigned)tok0 - (unsigned)v0, b = (unsigned)tok1 - (unsigned)v0;
+    if (rej0 && a < VC) atomicOr(&L.gone[a >> 5], 1u << (a & 31));
+    if (rej1 && b < VC) atomicOr(&L.gone[b >> 5], 1u << (b & 31));
   }
   __syncthreads();
-  int at = -1, count = 0, n_gone = 0;
+}
+
+__global__ void __launch_bounds__(VB) k_tree_verify(verify_args A) {
+  __shared__ verify_lds L;
+  __shared__ int s_path[DSH_TREE_MAX];
+  const int n = A.n, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, blocks = gridDim.x, me = blockIdx.x;
+  const int lo = me * A.share, hi = min(lo + A.share, A.vocab);
+  // node lane and node lane + 64
+  int par0 = -2, par1 = -2, tok0 = -1, tok1 = -1;
+  float u0 = 0.0f, u1 = 0.0f;
+  double p0 = 0.0, p1 = 0.0, q0 = 0.0, q1 = 0.0;
+  if (lane < n) {
+    par0 = A.parents[lane];
+    tok0 = A.tokens[lane];
+    u0 = A.u[lane];
+    if (par0 < -1 || par0 >= lane) par0 = -2;
+  }
+  if (lane + 64 < n) {
+    par1 = A.parents[lane + 64];
+    tok1 = A.tokens[lane + 64];
+    u1 = A.u[lane + 64];
+    if (par1 < -1 || par1 >= lane + 64) par1 = -2;
+  }
+  const float u_last = A.u[n];
+  if (par0 > -2 && tok0 >= 0 && tok0 < A.vocab) {
+    p0 = prob(A.p[(par0 + 1) * A.p_stride + tok0]);
+    if (A.q) q0 = prob(A.q[(par0 + 1) * A.q_stride + tok0]);
+  }
+  if (par1 > -2 && tok1 >= 0 && tok1 < A.vocab) {
+    p1 = prob(A.p[(par1 + 1) * A.p_stride + tok1]);
+    if (A.q) q1 = prob(A.q[(par1 + 1) * A.q_stride + tok1]);
+  }
+
+  int at = -1, count = 0, rounds = 0;
   double c = 0.0, z = 1.0, spent = 0.0;
-  for (int k = 0; k < n; k++) {  // children come after their parents
-    if (s_par[k] != at) continue;
-    const int tok = s_tok[k];
+  bool summed = false;  // L.sum holds the blocks' shares of what is left at the present context
+  // Sum of what is left over the row; every block's share in L.sum.
+  const auto row_sum = [&](const float *p, const float *q, bool marks) {
+    double mine = 0.0;
+    for (int v0 = lo; v0 < hi; v0 += VC) {
+      if (marks) verify_mark(L, v0, tok0, par0 == at, tok1, par1 == at);
+      const int v = v0 + 8 * tid;
+      double w[8];
+      if (v < hi) {
+        verify_left(w, p, q, c, v, hi, marks ? L.gone[tid >> 2] >> (8 * (tid & 3)) : 0);
+#pragma unroll
+        for (int e = 0; e < 8; e++) mine += w[e];
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) mine += __shfl_xor(mine, o);
+    if (lane == 0) L.part[wave] = mine;
+    if (tid == 0) L.fail = 0;
+    __syncthreads();
+    mine = (L.part[0] + L.part[1]) + (L.part[2] + L.part[3]);
+    if (wave == 0) {
+      u64 *w = A.words + (size_t)rounds * 128;
+      const u64 tag = (u64)A.epoch << 32, x = (u64)__double_as_longlong(mine);
+      if (blocks > 1 && lane < 2)
+        __hip_atomic_store(w + 2 * me + lane, tag | (lane ? x >> 32 : x & 0xFFFFFFFFu), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      double all = lane == me ? mine : 0.0;
+      if (blocks > 1) {
+        const u64 t0 = __builtin_amdgcn_s_memrealtime();
+        bool have = lane >= blocks || lane == me;
+        while (!__all(have)) {
+          if (!have) {
+            const u64 a = __hip_atomic_load(w + 2 * lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const u64 b = __hip_atomic_load(w + 2 * lane + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            have = (a >> 32) == A.epoch && (b >> 32) == A.epoch;
+            if (have) all = __longlong_as_double((long long)(b << 32 | (a & 0xFFFFFFFFu)));
+          }
+          __builtin_amdgcn_s_sleep(1);
+          if (__builtin_amdgcn_s_memrealtime() - t0 > VERIFY_TICKS) {
+            if (lane == 0) L.fail = 1;
+            break;
+          }
+        }
+      }
+      L.sum[lane] = all;
+    }
+    rounds++;
+    __syncthreads();
+    double s = 0.0;
+    for (int b = 0; b < blocks; b++) s += L.sum[b];
+    summed = true;
+    return s;
+  };
+
+  u64 m0 = __ballot(par0 == at), m1 = __ballot(par1 == at);
+  bool failed = false;
+  while ((m0 | m1) && !failed) {
+    const bool first = m0 != 0;
+    const int k = first ? __builtin_ctzll(m0) : __builtin_ctzll(m1);
+    if (first)
+      m0 &= m0 - 1;
+    else
+      m1 &= m1 - 1;
+    const double pk = read64(first ? p0 : p1, k), u = (double)dsh_readlane(first ? u0 : u1, k);
     bool hit;
-    if (A.target) {
-      hit = tok == A.target[at + 1];
-    } else if (tok < 0 || tok >= A.vocab) {
-      hit = false;
-      if (A.q) {
+    if (A.q) {
+      const double qk = read64(first ? q0 : q1, k), r = fmax(pk - c * qk, 0.0);
+      hit = r > 0.0 && u * qk * z < r;
+      if (!hit) {
         c += z;
-        z = residual_sum(residual{A.p + (at + 1) * A.p_stride, A.q + (at + 1) * A.q_stride, c, s_gone, 0}, 0, A.vocab, s_w);
+        z = row_sum(A.p + (at + 1) * A.p_stride, A.q + (at + 1) * A.q_stride, false);
+        failed = L.fail;
       }
     } else {
-      const float *p = A.p + (at + 1) * A.p_stride;
-      const double u = (double)A.u[k];
-      if (A.q) {
-        const float *q = A.q + (at + 1) * A.q_stride;
-        const double qt = prob(q[tok]), r = fmax(prob(p[tok]) - c * qt, 0.0);
-        hit = r > 0.0 && u * qt * z < r;
-        if (!hit) {
-          c += z;
-          z = residual_sum(residual{p, q, c, s_gone, 0}, 0, A.vocab, s_w);
-        }
-      } else {
-        double r = prob(p[tok]);
-        for (int g = 0; g < n_gone; g++)
-          if (s_gone[g] == tok) r = 0.0;
-        hit = r > 0.0 && u * (1.0 - spent) < r;
-        if (!hit) {
-          __syncthreads();
-          if (tid == 0) s_gone[n_gone] = tok;
-          __syncthreads();
-          n_gone++;
-          spent += r;
-        }
+      hit = pk > 0.0 && u * (1.0 - spent) < pk;
+      if (!hit) {
+        spent += pk;
+        const int t = __builtin_amdgcn_readlane(first ? tok0 : tok1, k);
+        if (par0 == at && tok0 == t) p0 = 0.0;  // nothing is left of the token for the next siblings
+        if (par1 == at && tok1 == t) p1 = 0.0;
       }
     }
     if (hit) {
-      if (tid == 0) A.path[count] = k;
+      at = first ? k : k + 64;
+      if (tid == 0) s_path[count] = at;
       count++;
-      at = k;
-      n_gone = 0;
-      c = 0.0;
+      c = spent = 0.0;
       z = 1.0;
-      spent = 0.0;
+      summed = false;
+      m0 = __ballot(par0 == at);
+      m1 = __ballot(par1 == at);
     }
   }
-  if (tid == 0) A.result[0] = count;
-  if (A.target) {
-    if (tid == 0) A.result[1] = A.target[at + 1];
-    return;
+
+  const float *p = A.p + (at + 1) * A.p_stride, *q = A.q && c > 0.0 ? A.q + (at + 1) * A.q_stride : nullptr;
+  bool marks = !A.q && __ballot(par0 == at || par1 == at);
+  double total = failed ? 0.0 : summed ? z : row_sum(p, q, marks);
+  if (!(total > 0.0) && (q || marks) && !failed && !L.fail) {  // nothing is left: p itself
+    q = nullptr;
+    marks = false;
+    total = row_sum(p, q, false);
   }
-  residual r{A.p + (at + 1) * A.p_stride, A.q ? A.q + (at + 1) * A.q_stride : nullptr, c, s_gone, n_gone};
-  double total = residual_sum(r, 0, A.vocab, s_w);
-  if (!(total > 0.0)) {
-    r.q = nullptr;
-    r.n_gone = 0;
-    total = residual_sum(r, 0, A.vocab, s_w);
-  }
-  if (!(total > 0.0)) {
-    if (tid == 0) A.result[1] = -1;
-    return;
-  }
-  // the piece of VT values that the threshold falls in, then the value
-  const double t = (double)A.u[n] * total;
-  double cum = 0.0;
-  int last = -1;  // the last piece with anything in it
-  for (int lo = 0; lo < A.vocab; lo += VT) {
-    const double s = residual_sum(r, lo, min(lo + VT, A.vocab), s_w);
-    if (s > 0.0) last = lo;
-    if (s > 0.0 && cum + s > t) break;
-    if (lo + VT < A.vocab) cum += s;
-  }
-  if (tid == 0) {
-    double a = cum;
-    int pick = -1;
-    for (int v = last; v < min(last + VT, A.vocab); v++) {
-      const double w = r.at(v);
-      if (!(w > 0.0)) continue;
-      pick = v;
-      a += w;
-      if (a > t) break;
+  failed = failed || (summed && L.fail);
+  if (me == 0) {
+    __syncthreads();
+    if (tid < n) A.path[tid] = tid < count && !failed ? s_path[tid] : -1;
+    if (tid == 0) {
+      A.result[0] = failed ? 0 : count;
+      if (failed || !(total > 0.0)) A.result[1] = -1;
+      if (failed && A.derr) __hip_atomic_store(A.derr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
     }
-    A.result[1] = pick;
   }
+  if (failed || !(total > 0.0)) return;
+  // the first block whose share crosses the threshold (for a number beyond [0, 1) the last with anything in it)
+  const double t = (double)u_last * total;
+  double before = 0.0, cum = 0.0;
+  int owner = -1, last = 0;
+  for (int b = 0; b < blocks && owner < 0; b++) {
+    const double s = L.sum[b];
+    if (s > 0.0) {
+      last = b;
+      if (cum + s > t) owner = b;
+    }
+    if (b == me) before = cum;
+    cum += s;
+  }
+  if (me != (owner < 0 ? last : owner)) return;
+  if (tid == 0) L.last = -1;
+  for (int v0 = lo; v0 < hi; v0 += VC) {
+    if (marks) verify_mark(L, v0, tok0, par0 == at, tok1, par1 == at);
+    const int v = v0 + 8 * tid;
+    double w[8], mine = 0.0;
+    int end = -1;
+#pragma unroll
+    for (int e = 0; e < 8; e++) w[e] = 0.0;
+    if (v < hi) verify_left(w, p, q, c, v, hi, marks ? L.gone[tid >> 2] >> (8 * (tid & 3)) : 0);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      mine += w[e];
+      if (w[e] > 0.0) end = v + e;
+    }
+    double x = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double y = __shfl_up(x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) L.part[wave] = x;
+    if (tid == 0) L.found = VB;
+    __syncthreads();
+    double b = before;
+#pragma unroll
+    for (int k = 0; k < VB / 64; k++) {
+      if (k < wave) b += L.part[k];
+      before += L.part[k];
+    }
+    if (end >= 0) atomicMax(&L.last, end);
+    if (mine > 0.0 && b + x > t) atomicMin(&L.found, tid);
+    __syncthreads();
+    if (L.found < VB) {
+      if (tid == L.found) {
+        double a = b + (x - mine);
+        int pick = end;
+#pragma unroll
+        for (int e = 7; e >= 0; e--) {  // from the back, so that the first that crosses stays
+          double y = a;
+#pragma unroll
+          for (int f = 0; f <= e; f++) y += w[f];
+          if (w[e] > 0.0 && y > t) pick = v + e;
+        }
+        A.result[1] = pick;
+      }
+      return;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) A.result[1] = L.last;
+}
+
+// Greedy: one wave, a node a lane, twice.
+__global__ void __launch_bounds__(64) k_tree_verify_greedy(int *path, int *result, const int *target, const int *tokens,
+                                                           const int *parents, int n) {
+  const int lane = threadIdx.x;
+  int par0 = -2, par1 = -2, next0 = 0, next1 = 0;
+  bool ok0 = false, ok1 = false;
+  const int root = target[0];
+  if (lane < n) {
+    par0 = parents[lane];
+    if (par0 < -1 || par0 >= lane) par0 = -2;
+    next0 = target[lane + 1];
+    ok0 = par0 > -2 && tokens[lane] == target[max(par0, -1) + 1];
+  }
+  if (lane + 64 < n) {
+    par1 = parents[lane + 64];
+    if (par1 < -1 || par1 >= lane + 64) par1 = -2;
+    next1 = target[lane + 65];
+    ok1 = par1 > -2 && tokens[lane + 64] == target[max(par1, -1) + 1];
+  }
+  int at = -1, count = 0, got0 = -1, got1 = -1;  // got: the path's entries lane and lane + 64
+  while (true) {
+    const u64 m0 = __ballot(ok0 && par0 == at), m1 = __ballot(ok1 && par1 == at);
+    if (!(m0 | m1)) break;
+    at = m0 ? __builtin_ctzll(m0) : 64 + __builtin_ctzll(m1);
+    if (lane == count) got0 = at;
+    if (lane + 64 == count) got1 = at;
+    count++;
+  }
+  if (lane < n) path[lane] = got0;
+  if (lane + 64 < n) path[lane + 64] = got1;
+  if (lane == 0) result[0] = count;
+  const int token = at < 0 ? root : at < 64 ? __builtin_amdgcn_readlane(next0, at) : __builtin_amdgcn_readlane(next1, at & 63);
+  if (lane == 0) result[1] = token;
 }
 
 // ---------------------------------------------------------------------------- commit
@@ -755,11 +934,21 @@ hipError_t dsh_launch_tree_attention(const dsh_tree_attn_t *A, float *work, hipS
 }
 
 hipError_t dsh_launch_tree_verify(int *path, int *result, const float *p, int64_t p_stride, const float *q,
-                                  int64_t q_stride, int vocab, const int *target, const int *tokens, const int *parents,
-                                  int n_nodes, const float *u, hipStream_t s) {
+                                  int64_t q_stride, int vocab, const int *tokens, const int *parents, int n_nodes,
+                                  const float *u, unsigned long long *words, unsigned epoch, int *derr, hipStream_t s) {
+  if (n_nodes < 0 || n_nodes > DSH_TREE_MAX || vocab < 1) return hipErrorInvalidValue;
+  // a block per VC values, 64 at most (a lane each when the shares are told); shares in whole eights
+  const int want = (int)(((int64_t)vocab + VC - 1) / VC), blocks = want < 64 ? want : 64;
+  const int64_t share = (((int64_t)vocab + blocks - 1) / blocks + 7) / 8 * 8;
+  const verify_args a{path, result, p, q, u, tokens, parents, p_stride, q_stride, vocab, n_nodes, (int)share, words, epoch, derr};
+  k_tree_verify<<<(int)((vocab + share - 1) / share), VB, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t dsh_launch_tree_verify_greedy(int *path, int *result, const int *target, const int *tokens, const int *parents,
+                                         int n_nodes, hipStream_t s) {
   if (n_nodes < 0 || n_nodes > DSH_TREE_MAX) return hipErrorInvalidValue;
-  const verify_args a{path, result, p, q, u, target, tokens, parents, p_stride, q_stride, vocab, n_nodes};
-  k_tree_verify<<<1, VT, 0, s>>>(a);
+  k_tree_verify_greedy<<<1, 64, 0, s>>>(path, result, target, tokens, parents, n_nodes);
   return hipGetLastError();
 }
 

@@ -130,16 +130,27 @@ int ds_hip_tree_attention(float *out_dev, int64_t out_stride, float *lse_dev, fl
   return leave(dev, me, dsh_launch_tree_attention(&a, work, dsr_stream));
 }
 
-static int verify(const char *me, int *path_dev, int *result_dev, const float *p, int64_t p_stride, const float *q,
-                  int64_t q_stride, int vocab, const int *target, const int *tokens, const int *parents, int n_nodes,
-                  const float *u) {
+static int verify_check(const char *me, const int *path, const int *result, const int *tokens, const int *parents, int n_nodes) {
   if (n_nodes < 0 || n_nodes > DS_HIP_TREE_MAX_NODES)
     return dsr_failf("%s: %d nodes (0 to %d)", me, n_nodes, DS_HIP_TREE_MAX_NODES);
-  if (!result_dev || (n_nodes && (!path_dev || !tokens || !parents))) return dsr_failf("%s: NULL argument", me);
-  int dev;
-  if (enter(&dev)) return -1;
-  return leave(dev, me, dsh_launch_tree_verify(path_dev, result_dev, p, p_stride, q, q_stride, vocab, target, tokens, parents,
-                                               n_nodes, u, dsr_stream));
+  if (!result || (n_nodes && (!path || !tokens || !parents))) return dsr_failf("%s: NULL argument", me);
+  return 0;
+}
+
+/* The words that a verification's blocks tell each other their sums in: zeroed once, every launch with an epoch of its own. */
+static unsigned long long *verify_words(void) {
+  static void *words = NULL;
+  if (words) return (unsigned long long *)words;
+  const size_t bytes = (size_t)DSH_VERIFY_WORDS * 8;
+  void *p = NULL;
+  hipError_t e = hipMalloc(&p, bytes);
+  if (e == hipSuccess) e = hipMemsetAsync(p, 0, bytes, dsr_stream);
+  if (e != hipSuccess) {
+    dsr_fail("verification words", e);
+    if (p) hipFree(p);
+    return NULL;
+  }
+  return (unsigned long long *)(words = p);
 }
 
 int ds_hip_tree_verify(int *path_dev, int *result_dev, const float *p_dev, int64_t p_stride, const float *q_dev,
@@ -147,18 +158,31 @@ int ds_hip_tree_verify(int *path_dev, int *result_dev, const float *p_dev, int64
                        const float *u_dev) {
   static const char *const me = "ds_hip_tree_verify";
   if (!p_dev || !u_dev) return dsr_failf("%s: NULL argument", me);
+  if (verify_check(me, path_dev, result_dev, tokens_dev, parents_dev, n_nodes)) return -1;
   if (vocab < 1 || (n_nodes > 0 && (p_stride < vocab || (q_dev && q_stride < vocab))) || p_stride > STRIDE_MAX ||
       q_stride > STRIDE_MAX)
     return dsr_failf("%s: vocab %d, strides %lld and %lld", me, vocab, (long long)p_stride, (long long)q_stride);
-  return verify(me, path_dev, result_dev, p_dev, p_stride, q_dev, q_stride, vocab, NULL, tokens_dev, parents_dev, n_nodes,
-                u_dev);
+  int dev;
+  if (enter(&dev)) return -1;
+  unsigned long long *words = verify_words();
+  if (!words) {
+    leave(dev, me, hipSuccess);
+    return -1;
+  }
+  return leave(dev, me, dsh_launch_tree_verify(path_dev, result_dev, p_dev, p_stride, q_dev, q_stride, vocab, tokens_dev,
+                                               parents_dev, n_nodes, u_dev, words, dsr_expert_epoch(),
+                                               dsr_derr_dev(DSR_DERR_VERIFY_WAIT), dsr_stream));
 }
 
 int ds_hip_tree_verify_greedy(int *path_dev, int *result_dev, const int *target_dev, const int *tokens_dev,
                               const int *parents_dev, int n_nodes) {
   static const char *const me = "ds_hip_tree_verify_greedy";
   if (!target_dev) return dsr_failf("%s: NULL argument", me);
-  return verify(me, path_dev, result_dev, NULL, 0, NULL, 0, 0, target_dev, tokens_dev, parents_dev, n_nodes, NULL);
+  if (verify_check(me, path_dev, result_dev, tokens_dev, parents_dev, n_nodes)) return -1;
+  int dev;
+  if (enter(&dev)) return -1;
+  return leave(dev, me, dsh_launch_tree_verify_greedy(path_dev, result_dev, target_dev, tokens_dev, parents_dev, n_nodes,
+                                                      dsr_stream));
 }
 
 int ds_hip_tree_commit(const ds_hip_kv_t *cache, int n_cache, const ds_hip_kv_t *tree, int n_nodes, const int *path_dev,

@@ -30,7 +30,7 @@ int dsr_failf(const char *fmt, ...);
  * dsr_init). dsr_derr_check() reports (and clears) any word that is set: -1 with ds_hip_last_error
  * naming the failure, else 0. It runs after every synchronisation the library API offers
  * (ds_hip_sync) and at the entry of the calls whose results such a failure voids. */
-enum { DSR_DERR_PREFILL_WAIT, DSR_DERR_ROUTE_WAIT, DSR_DERR_EXPERT_WAIT, DSR_DERR_N };
+enum { DSR_DERR_PREFILL_WAIT, DSR_DERR_ROUTE_WAIT, DSR_DERR_EXPERT_WAIT, DSR_DERR_VERIFY_WAIT, DSR_DERR_N };
 int *dsr_derr_dev(int kind);
 int dsr_derr_check(void);
 

@@ -84,6 +84,7 @@ int dsr_derr_check(void) {
       "decode: a certified layer's bounded wait for its verdict on the expert selection gave up; the "
       "step's output is not valid",
       "expert: the down rows' bounded wait for the gate_up rows' h gave up; that call's output is not valid",
+      "tree verification: a block's bounded wait for the other blocks' sums gave up; that call's output is not valid",
   };
   if (!g_derr_host) return 0;
   int rc = 0;

@@ -480,7 +480,8 @@ def evict_case(dev, G, D, n, keep, bf16=False, by_head=False, sink=0, recent=Non
 
 
 @pytest.mark.parametrize("n, keep", [(1, 1), (2, 1), (5, 5), (64, 63), (65, 1), (100, 37), (1023, 512), (1024, 1000), (1025, 1024),
-                                     (3000, 1500), (3001, 2999), (7679, 4096), (20000, 9000)])
+                                     (3000, 1500), (3001, 2999), (4096, 4000), (4097, 100), (7679, 4096), (8193, 8000), (16384, 5000),
+                                     (20000, 9000), (32768, 16384), (32769, 16384), (70001, 30000)])
 def test_evict_lengths(dev, n, keep):
     evict_case(dev, 3, 64, n, keep, seed=n)
     evict_case(dev, 2, 128, n, keep, bf16=True, by_head=True, sink=3, recent=max(0, n - n // 4), in_place=True, seed=n + 1)
