@@ -519,8 +519,27 @@ __device__ __forceinline__ double read64(double v, int lane) {
 struct verify_lds {
   double part[VB / 64], sum[64];
   unsigned gone[VC / 32];
-  int found, last, fail;
+  int fail;
 };
+
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {  // 0 where a lane has no source
+  const u64 x = (u64)__double_as_longlong(v);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)x, CTRL, 0xF, 0xF, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(x >> 32), CTRL, 0xF, 0xF, false);
+  return __longlong_as_double((long long)((u64)hi << 32 | lo));
+}
+// Sum over the lanes up to this one; *total: over all.
+__device__ __forceinline__ double wave_scan64(double v, double *total) {
+  v += dpp64<0x111>(v);  // row_shr:1, 2, 4, 8
+  v += dpp64<0x112>(v);
+  v += dpp64<0x114>(v);
+  v += dpp64<0x118>(v);
+  const double r1 = read64(v, 15), r2 = r1 + read64(v, 31), r3 = r2 + read64(v, 47);
+  *total = r3 + read64(v, 63);
+  const int row = (threadIdx.x >> 4) & 3;
+  return row == 0 ? v : (row == 1 ? r1 : row == 2 ? r2 : r3) + v;
+}
 
 // What is left of the thread's eight values from v on: max(p - c q, 0), or p without the rejected tokens (bits of gone).
 __device__ __forceinline__ void verify_left(double *w, const float *p, const float *q, double c, int v, int end, unsigned gone) {
@@ -596,42 +615,40 @@ __global__ void __launch_bounds__(VB) k_tree_verify(verify_args A) {
   int at = -1, count = 0, rounds = 0;
   double c = 0.0, z = 1.0, spent = 0.0;
   bool summed = false;  // L.sum holds the blocks' shares of what is left at the present context
-  // Sum of what is left over the row; every block's share in L.sum.
+  // What is left of the row: every block's share in L.sum, their sum; w: the thread's own values of the last piece
+  double w[8];
+  const auto load = [&](const float *p, const float *q, bool marks, int v0) {
+    if (marks) verify_mark(L, v0, tok0, par0 == at, tok1, par1 == at);
+    const int v = v0 + 8 * tid;
+#pragma unroll
+    for (int e = 0; e < 8; e++) w[e] = 0.0;
+    if (v < hi) verify_left(w, p, q, c, v, hi, marks ? L.gone[tid >> 2] >> (8 * (tid & 3)) : 0);
+    return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+  };
   const auto row_sum = [&](const float *p, const float *q, bool marks) {
     double mine = 0.0;
-    for (int v0 = lo; v0 < hi; v0 += VC) {
-      if (marks) verify_mark(L, v0, tok0, par0 == at, tok1, par1 == at);
-      const int v = v0 + 8 * tid;
-      double w[8];
-      if (v < hi) {
-        verify_left(w, p, q, c, v, hi, marks ? L.gone[tid >> 2] >> (8 * (tid & 3)) : 0);
-#pragma unroll
-        for (int e = 0; e < 8; e++) mine += w[e];
-      }
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) mine += __shfl_xor(mine, o);
+    for (int v0 = lo; v0 < hi; v0 += VC) mine += load(p, q, marks, v0);
+    wave_scan64(mine, &mine);
     if (lane == 0) L.part[wave] = mine;
     if (tid == 0) L.fail = 0;
     __syncthreads();
-    mine = (L.part[0] + L.part[1]) + (L.part[2] + L.part[3]);
     if (wave == 0) {
-      u64 *w = A.words + (size_t)rounds * 128;
+      mine = ((L.part[0] + L.part[1]) + L.part[2]) + L.part[3];
+      u64 *t = A.words + (size_t)rounds * 128;
       const u64 tag = (u64)A.epoch << 32, x = (u64)__double_as_longlong(mine);
       if (blocks > 1 && lane < 2)
-        __hip_atomic_store(w + 2 * me + lane, tag | (lane ? x >> 32 : x & 0xFFFFFFFFu), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(t + 2 * me + lane, tag | (lane ? x >> 32 : x & 0xFFFFFFFFu), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       double all = lane == me ? mine : 0.0;
       if (blocks > 1) {
         const u64 t0 = __builtin_amdgcn_s_memrealtime();
         bool have = lane >= blocks || lane == me;
         while (!__all(have)) {
           if (!have) {
-            const u64 a = __hip_atomic_load(w + 2 * lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const u64 b = __hip_atomic_load(w + 2 * lane + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const u64 a = __hip_atomic_load(t + 2 * lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const u64 b = __hip_atomic_load(t + 2 * lane + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             have = (a >> 32) == A.epoch && (b >> 32) == A.epoch;
             if (have) all = __longlong_as_double((long long)(b << 32 | (a & 0xFFFFFFFFu)));
           }
-          __builtin_amdgcn_s_sleep(1);
           if (__builtin_amdgcn_s_memrealtime() - t0 > VERIFY_TICKS) {
             if (lane == 0) L.fail = 1;
             break;
@@ -642,14 +659,16 @@ __global__ void __launch_bounds__(VB) k_tree_verify(verify_args A) {
     }
     rounds++;
     __syncthreads();
-    double s = 0.0;
-    for (int b = 0; b < blocks; b++) s += L.sum[b];
+    double s;
+    wave_scan64(L.sum[lane], &s);
     summed = true;
     return s;
   };
 
   u64 m0 = __ballot(par0 == at), m1 = __ballot(par1 == at);
-  bool failed = false;
+  // a context's first child is tried against p itself: all of those tests at once
+  const u64 h0 = __ballot(p0 > 0.0 && (double)u0 * (A.q ? q0 : 1.0) < p0), h1 = __ballot(p1 > 0.0 && (double)u1 * (A.q ? q1 : 1.0) < p1);
+  bool failed = false, fresh = true;
   while ((m0 | m1) && !failed) {
     const bool first = m0 != 0;
     const int k = first ? __builtin_ctzll(m0) : __builtin_ctzll(m1);
@@ -657,24 +676,27 @@ __global__ void __launch_bounds__(VB) k_tree_verify(verify_args A) {
       m0 &= m0 - 1;
     else
       m1 &= m1 - 1;
-    const double pk = read64(first ? p0 : p1, k), u = (double)dsh_readlane(first ? u0 : u1, k);
-    bool hit;
-    if (A.q) {
-      const double qk = read64(first ? q0 : q1, k), r = fmax(pk - c * qk, 0.0);
-      hit = r > 0.0 && u * qk * z < r;
-      if (!hit) {
-        c += z;
-        z = row_sum(A.p + (at + 1) * A.p_stride, A.q + (at + 1) * A.q_stride, false);
-        failed = L.fail;
+    bool hit = ((first ? h0 : h1) >> k) & 1;
+    if (!fresh || !hit) {
+      const double pk = read64(first ? p0 : p1, k), u = (double)dsh_readlane(first ? u0 : u1, k);
+      if (A.q) {
+        const double qk = read64(first ? q0 : q1, k), r = fmax(pk - c * qk, 0.0);
+        hit = r > 0.0 && u * qk * z < r;
+        if (!hit) {
+          c += z;
+          z = row_sum(A.p + (at + 1) * A.p_stride, A.q + (at + 1) * A.q_stride, false);
+          failed = L.fail;
+        }
+      } else {
+        hit = pk > 0.0 && u * (1.0 - spent) < pk;
+        if (!hit) {
+          spent += pk;
+          const int t = __builtin_amdgcn_readlane(first ? tok0 : tok1, k);
+          if (par0 == at && tok0 == t) p0 = 0.0;  // nothing is left of the token for the next siblings
+          if (par1 == at && tok1 == t) p1 = 0.0;
+        }
       }
-    } else {
-      hit = pk > 0.0 && u * (1.0 - spent) < pk;
-      if (!hit) {
-        spent += pk;
-        const int t = __builtin_amdgcn_readlane(first ? tok0 : tok1, k);
-        if (par0 == at && tok0 == t) p0 = 0.0;  // nothing is left of the token for the next siblings
-        if (par1 == at && tok1 == t) p1 = 0.0;
-      }
+      fresh = false;
     }
     if (hit) {
       at = first ? k : k + 64;
@@ -683,6 +705,7 @@ __global__ void __launch_bounds__(VB) k_tree_verify(verify_args A) {
       c = spent = 0.0;
       z = 1.0;
       summed = false;
+      fresh = true;
       m0 = __ballot(par0 == at);
       m1 = __ballot(par1 == at);
     }
@@ -707,71 +730,57 @@ __global__ void __launch_bounds__(VB) k_tree_verify(verify_args A) {
     }
   }
   if (failed || !(total > 0.0)) return;
-  // the first block whose share crosses the threshold (for a number beyond [0, 1) the last with anything in it)
-  const double t = (double)u_last * total;
-  double before = 0.0, cum = 0.0;
-  int owner = -1, last = 0;
-  for (int b = 0; b < blocks && owner < 0; b++) {
-    const double s = L.sum[b];
-    if (s > 0.0) {
-      last = b;
-      if (cum + s > t) owner = b;
-    }
-    if (b == me) before = cum;
-    cum += s;
-  }
-  if (me != (owner < 0 ? last : owner)) return;
-  if (tid == 0) L.last = -1;
+  // the first block whose share crosses the threshold (for a number beyond [0, 1) the last with anything in it), then the
+  // wave, the lane and the value
+  const double t = (double)u_last * total, share = L.sum[lane];
+  double all, before = wave_scan64(share, &all) - share;
+  const auto pick = [](u64 crosses, u64 filled) { return crosses ? __builtin_ctzll(crosses) : 63 - __builtin_clzll(filled); };
+  if (me != pick(__ballot(share > 0.0 && before + share > t), __ballot(share > 0.0))) return;
+  before = read64(before, me);
+  int last = -1;
   for (int v0 = lo; v0 < hi; v0 += VC) {
-    if (marks) verify_mark(L, v0, tok0, par0 == at, tok1, par1 == at);
-    const int v = v0 + 8 * tid;
-    double w[8], mine = 0.0;
-    int end = -1;
-#pragma unroll
-    for (int e = 0; e < 8; e++) w[e] = 0.0;
-    if (v < hi) verify_left(w, p, q, c, v, hi, marks ? L.gone[tid >> 2] >> (8 * (tid & 3)) : 0);
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      mine += w[e];
-      if (w[e] > 0.0) end = v + e;
-    }
-    double x = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_up(x, o);
-      if (lane >= o) x += y;
-    }
+    const double mine = hi - lo > VC ? load(p, q, marks, v0) : ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    double sum, x = wave_scan64(mine, &sum);
     __syncthreads();
-    if (lane == 63) L.part[wave] = x;
-    if (tid == 0) L.found = VB;
+    if (lane == 0) L.part[wave] = sum;
     __syncthreads();
-    double b = before;
+    double base = before;
+    int own = -1;
 #pragma unroll
     for (int k = 0; k < VB / 64; k++) {
-      if (k < wave) b += L.part[k];
+      if (k == wave) base = before;
       before += L.part[k];
+      if (own < 0 && L.part[k] > 0.0 && before > t) own = k;
     }
-    if (end >= 0) atomicMax(&L.last, end);
-    if (mine > 0.0 && b + x > t) atomicMin(&L.found, tid);
-    __syncthreads();
-    if (L.found < VB) {
-      if (tid == L.found) {
-        double a = b + (x - mine);
-        int pick = end;
 #pragma unroll
-        for (int e = 7; e >= 0; e--) {  // from the back, so that the first that crosses stays
-          double y = a;
+    for (int e = 0; e < 8; e++)
+      if (w[e] > 0.0) last = v0 + 8 * tid + e;
+    if (own < 0) continue;
+    if (own != wave) return;
+    const int k = pick(__ballot(mine > 0.0 && base + x > t), __ballot(mine > 0.0));
+    if (lane == k) {
+      double a = base + (x - mine);
+      int token = -1;
+      bool done = false;
 #pragma unroll
-          for (int f = 0; f <= e; f++) y += w[f];
-          if (w[e] > 0.0 && y > t) pick = v + e;
+      for (int e = 0; e < 8; e++) {
+        a += w[e];
+        if (w[e] > 0.0 && !done) {
+          token = v0 + 8 * tid + e;
+          done = a > t;
         }
-        A.result[1] = pick;
       }
-      return;
+      A.result[1] = token;
     }
+    return;
   }
+  // no more than a rounding is missing (or the number lies beyond [0, 1)): the last value with anything in it
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) last = max(last, __shfl_xor(last, o));
   __syncthreads();
-  if (tid == 0) A.result[1] = L.last;
+  if (lane == 0) s_path[wave] = last;
+  __syncthreads();
+  if (tid == 0) A.result[1] = max(max(s_path[0], s_path[1]), max(s_path[2], s_path[3]));
 }
 
 // Greedy: one wave, a node a lane, twice.

@@ -314,6 +314,22 @@ def test_verify_full_vocabulary(dev, n, drawn):
                                                                                      parents, V), seed
 
 
+@pytest.mark.parametrize("drawn", [False, True])
+def test_verify_large_vocabulary(dev, drawn):
+    """More than one piece a block; the weight in the last values, in the first, in none of a block's last piece."""
+    V, n = 300000, 2
+    rng = np.random.default_rng(9)
+    for where in (slice(0, V), slice(0, 3), slice(V - 3, V), slice(150000, 150001), slice(2040, 2060)):
+        p = np.zeros((n + 1, V), np.float32)
+        p[:, where] = rng.random(p[:, where].shape, dtype=np.float32) + 1e-3
+        p /= p.sum(1, keepdims=True)
+        q = np.full((n + 1, V), 1 / V, np.float32)
+        for last in (0.0, 0.3, 1 - 2 ** -24):
+            u = np.array([0.9, 0.9, last], np.float32)
+            tokens, parents = np.array([5, V - 1], np.int32), np.array([-1, -1], np.int32)
+            assert verify(dev, p, q if drawn else None, u, tokens, parents, V) == R.verify(p, q if drawn else None, u, tokens, parents, V)
+
+
 def test_verify_borders_and_strange_values(dev):
     """Equal sides are a rejection; NaN, infinite, negative and zero probabilities; nothing left; a token twice."""
     V, n = 8, 3
