@@ -5,6 +5,7 @@
 
 #define ET 1024
 #define EW (ET / 64)
+#define EVICT_OWN 131072  // bytes of K and V rows of a head
 
 typedef unsigned long long u64;
 
@@ -21,39 +22,86 @@ __device__ __forceinline__ uint32_t evict_number(float a, bool guarded, bool spi
   return guarded == spill ? evict_key(a) : spill ? 0u : 0xFFFFFFFFu;
 }
 
-// Three counts of a wave (the same in all its lanes) summed over the block.
-__device__ __forceinline__ void evict_sums(int (*s_cnt)[EW], int &a, int &b, int &c) {
+// Sum over the block of three counts (each a wave's, the same in all its lanes), by way of s (3 x EW words, not in use by
+// the call before this one).
+__device__ __forceinline__ void evict_sums(int (*s)[EW], int &a, int &b, int &c) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane < 3) s[lane][wave] = lane == 0 ? a : lane == 1 ? b : c;
   __syncthreads();
-  if (lane < 3) s_cnt[lane][wave] = lane == 0 ? a : lane == 1 ? b : c;
-  __syncthreads();
-  int x = lane < 48 ? s_cnt[lane >> 4][lane & 15] : 0;
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o);
+  int x = lane < 48 ? s[lane >> 4][lane & 15] : 0;
+  x += __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false);   // over the 16 lanes of a row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x141, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x140, 0xF, 0xF, false);
   a = __builtin_amdgcn_readlane(x, 0);
   b = __builtin_amdgcn_readlane(x, 16);
   c = __builtin_amdgcn_readlane(x, 32);
 }
 
-// The gone-th lowest number T, two bits at a step: each counts the numbers below three candidates by wave votes (count(t)
-// is a wave's), which costs the same whatever the numbers are; a histogram in LDS piles up on the few exponents that weights
-// have. left: how many of those equal to T go.
-template <typename F>
-__device__ __forceinline__ void evict_threshold(int (*s_cnt)[EW], int gone, uint32_t &T, int &left, F count) {
+struct evict_lds {
+  int cnt[2][3][EW];
+  uint32_t few[64], T;
+  int n_few, left, equal;
+};
+
+// The gone-th lowest number T, two bits at a step: each counts the numbers below three candidates by wave votes (count(t...)
+// adds a wave's), which costs the same whatever the numbers are; a histogram in LDS piles up on the few exponents that
+// weights have. Once at most 64 numbers are in question, gather(T, mask) puts them in few, and one wave ranks them. left: how
+// many of those equal to T go, equal: of how many.
+template <typename F, typename G>
+__device__ __forceinline__ void evict_threshold(evict_lds &L, int gone, int n, uint32_t &T, int &left, int &equal, F count,
+                                                G gather) {
   T = 0;
-  left = gone;
+  left = equal = 0;  // no number is 0 unless it goes
   if (gone == 0) return;
+  if (threadIdx.x == 0) L.n_few = 0;
+  int under = 0, over = n;  // numbers below T, and below T + 4^k
   for (int shift = 30; shift >= 0; shift -= 2) {
     const uint32_t t1 = T | 1u << shift, t2 = T | 2u << shift, t3 = T | 3u << shift;
     int c1 = 0, c2 = 0, c3 = 0;
     count(t1, t2, t3, c1, c2, c3);
-    evict_sums(s_cnt, c1, c2, c3);
-    const int c = c3 < gone ? c3 : c2 < gone ? c2 : c1;
-    if (c < gone) {
-      T = c3 < gone ? t3 : c2 < gone ? t2 : t1;
-      left = gone - c;
+    evict_sums(L.cnt[(shift >> 1) & 1], c1, c2, c3);
+    if (c3 < gone) {
+      T = t3;
+      under = c3;
+    } else if (c2 < gone) {
+      T = t2;
+      under = c2;
+      over = c3;
+    } else if (c1 < gone) {
+      T = t1;
+      under = c1;
+      over = c2;
+    } else {
+      over = c1;
+    }
+    if (shift > 0 && over - under <= 64) {
+      gather(T, ~0u << shift);
+      __syncthreads();
+      if (threadIdx.x < 64) {
+        const int lane = threadIdx.x, m = over - under;
+        const uint32_t k = lane < m ? L.few[lane] : 0xFFFFFFFFu;
+        int less = 0, leq = 0;
+        for (int x = 0; x < m; x++) {
+          const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)k, x);
+          less += o < k;
+          leq += o <= k;
+        }
+        if (lane < m && under + less < gone && under + leq >= gone) {  // equal lanes write the same
+          L.T = k;
+          L.left = gone - under - less;
+          L.equal = leq - less;
+        }
+      }
+      __syncthreads();
+      T = L.T;
+      left = L.left;
+      equal = L.equal;
+      return;
     }
   }
+  left = gone - under;
+  equal = over - under;
 }
 
 // Exclusive prefix of N cells (a multiple of 64) by one wave; s[N] becomes the sum.
@@ -68,11 +116,13 @@ __device__ __forceinline__ void evict_prefix(int *s) {
     sum += v[k];
   }
   int x = sum;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  const int r0 = __builtin_amdgcn_readlane(x, 15), r1 = r0 + __builtin_amdgcn_readlane(x, 31);
+  const int r2 = r1 + __builtin_amdgcn_readlane(x, 47);
+  x += lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r1 : r2;
   if (lane == 63) s[N] = x;
   x -= sum;
 #pragma unroll
@@ -82,13 +132,41 @@ __device__ __forceinline__ void evict_prefix(int *s) {
   }
 }
 
+// K and V rows of the movers into the holes, 16 bytes a thread, four pieces under way. P: 16-byte pieces of a row.
+__device__ __forceinline__ void evict_move(const dsh_kv_evict_t &A, int h, int count, const int *hole, const int *mover, int P,
+                                           int64_t first, int64_t step) {
+  const int64_t rs = A.cache.row_stride * (A.cache.bf16 ? 2 : 4), hs = A.cache.head_stride * (A.cache.bf16 ? 2 : 4);
+  char *k = (char *)A.cache.k + h * hs, *v = (char *)A.cache.v + h * hs;
+  const int64_t total = (int64_t)count * 2 * P;
+  for (int64_t x = first; x < total; x += 4 * step) {
+    u32x4 y[4];
+    char *to[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int64_t i = x + u * step;
+      to[u] = nullptr;
+      if (i < total) {
+        const int r = (int)((uint64_t)i / (unsigned)(2 * P)), piece = (int)(i - (int64_t)r * 2 * P);
+        char *b = piece < P ? k + 16 * piece : v + 16 * (piece - P);
+        to[u] = b + hole[r] * rs;
+        y[u] = *(const u32x4 *)(b + mover[r] * rs);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+      if (to[u]) *(u32x4 *)to[u] = y[u];
+  }
+}
+
 // One block per head, up to 1024 E rows in registers; thread t has the rows 1024 e + t. Ranks (among the equal numbers, then of
 // the holes below `keep` and of the rows that fill them) come from votes too: a count for every 64 rows, a prefix over those.
 // Workspace: per head a count, then holes [most] and movers [most], most = min(n - keep, keep).
+// move: the rows' own pieces, where the block itself moves them (0: k_kv_move does).
 template <int E>
-__global__ void __launch_bounds__(ET) k_kv_select(dsh_kv_evict_t A, int most) {
+__global__ void __launch_bounds__(ET) k_kv_select(dsh_kv_evict_t A, int most, int move) {
   constexpr int N = E * EW;
-  __shared__ int s_cnt[3][EW], s_a[N + 1], s_b[N + 1];
+  __shared__ evict_lds L;
+  __shared__ int s_a[N + 1], s_b[N + 1];
   extern __shared__ uint16_t s_mv[];  // [most]
   const int h = blockIdx.x, n = A.n, keep = A.keep, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -112,37 +190,47 @@ __global__ void __launch_bounds__(ET) k_kv_select(dsh_kv_evict_t A, int most) {
     guard |= (uint32_t)g << e;
     free_rows += __popcll(__ballot(ET * e + tid < n && !g));
   }
-  evict_sums(s_cnt, free_rows, none, none2);
+  evict_sums(L.cnt[0], free_rows, none, none2);  // the first step takes the other
   const int gone = n - keep;
   const bool spill = gone > free_rows;
 #pragma unroll
   for (int e = 0; e < E; e++)
     key[e] = ET * e + tid < n ? evict_number(__uint_as_float(key[e]), (guard >> e) & 1, spill) : 0xFFFFFFFFu;
   uint32_t T;
-  int left;
-  evict_threshold(s_cnt, gone, T, left, [&](uint32_t t1, uint32_t t2, uint32_t t3, int &c1, int &c2, int &c3) {
+  int left, equal;
+  const auto count_below = [&](uint32_t t1, uint32_t t2, uint32_t t3, int &c1, int &c2, int &c3) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
       c1 += __popcll(__ballot(key[e] < t1));
       c2 += __popcll(__ballot(key[e] < t2));
       c3 += __popcll(__ballot(key[e] < t3));
     }
+  };
+  evict_threshold(L, gone, n, T, left, equal, count_below, [&](uint32_t t, uint32_t mask) {
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      if (ET * e + tid < n && (key[e] & mask) == t) L.few[atomicAdd(&L.n_few, 1) & 63] = key[e];
   });
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const int c = __popcll(__ballot(key[e] == T));
-    if (lane == 0) s_a[e * EW + wave] = c;
-  }
-  __syncthreads();
-  if (wave == 0) evict_prefix<N>(s_a);
-  __syncthreads();
   uint32_t stays = 0;
+  if (left == equal) {
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    const int rank = s_a[e * EW + wave] + __popcll(__ballot(key[e] == T) & below);
-    stays |= (uint32_t)(ET * e + tid < n && (key[e] > T || (key[e] == T && rank >= left))) << e;
+    for (int e = 0; e < E; e++) stays |= (uint32_t)(ET * e + tid < n && key[e] > T) << e;
+  } else {  // ranks among the equal ones
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int c = __popcll(__ballot(key[e] == T));
+      if (lane == 0) s_a[e * EW + wave] = c;
+    }
+    __syncthreads();
+    if (wave == 0) evict_prefix<N>(s_a);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int rank = s_a[e * EW + wave] + __popcll(__ballot(key[e] == T) & below);
+      stays |= (uint32_t)(ET * e + tid < n && (key[e] > T || (key[e] == T && rank >= left))) << e;
+    }
+    __syncthreads();
   }
-  __syncthreads();
 #pragma unroll
   for (int e = 0; e < E; e++) {
     const int j = ET * e + tid;
@@ -182,11 +270,16 @@ __global__ void __launch_bounds__(ET) k_kv_select(dsh_kv_evict_t A, int most) {
       if (A.pos_out) A.pos_out[h * A.pos_out_stride + j] = pos[from];
     }
   }
+  if (move) {
+    __syncthreads();
+    evict_move(A, h, s_a[N], hole, mover, move, tid, ET);
+  }
 }
 
 // The same for more rows than that, read again at every step; a thread's rows are consecutive where ranks are counted.
 __global__ void __launch_bounds__(ET) k_kv_select_long(dsh_kv_evict_t A, int most) {
-  __shared__ int s_cnt[3][EW], s_a[ET + 1], s_b[ET + 1];
+  __shared__ evict_lds L;
+  __shared__ int s_a[ET + 1], s_b[ET + 1];
   const int h = blockIdx.x, n = A.n, keep = A.keep, tid = threadIdx.x;
   const float *acc = A.acc + h * A.acc_stride;
   const int *pos = A.pos ? A.pos + h * A.pos_stride : nullptr;
@@ -197,18 +290,24 @@ __global__ void __launch_bounds__(ET) k_kv_select_long(dsh_kv_evict_t A, int mos
   };
   int free_rows = 0, none = 0, none2 = 0;
   for (int j0 = 0; j0 < n; j0 += ET) free_rows += __popcll(__ballot(j0 + tid < n && !guarded(min(j0 + tid, n - 1))));
-  evict_sums(s_cnt, free_rows, none, none2);
+  evict_sums(L.cnt[0], free_rows, none, none2);  // the first step takes the other
   const int gone = n - keep;
   const bool spill = gone > free_rows;
   const auto number = [&](int j) { return evict_number(acc[j], guarded(j), spill); };
   uint32_t T;
-  int left;
-  evict_threshold(s_cnt, gone, T, left, [&](uint32_t t1, uint32_t t2, uint32_t t3, int &c1, int &c2, int &c3) {
+  int left, equal;
+  const auto count_below = [&](uint32_t t1, uint32_t t2, uint32_t t3, int &c1, int &c2, int &c3) {
     for (int j0 = 0; j0 < n; j0 += ET) {
       const uint32_t k = j0 + tid < n ? number(j0 + tid) : 0xFFFFFFFFu;
       c1 += __popcll(__ballot(k < t1));
       c2 += __popcll(__ballot(k < t2));
       c3 += __popcll(__ballot(k < t3));
+    }
+  };
+  evict_threshold(L, gone, n, T, left, equal, count_below, [&](uint32_t t, uint32_t mask) {
+    for (int j = tid; j < n; j += ET) {
+      const uint32_t k = number(j);
+      if ((k & mask) == t) L.few[atomicAdd(&L.n_few, 1) & 63] = k;
     }
   });
   const int per = (int)(((int64_t)n + ET - 1) / ET);
@@ -264,32 +363,11 @@ __global__ void __launch_bounds__(ET) k_kv_select_long(dsh_kv_evict_t A, int mos
   }
 }
 
-// K and V rows of the movers into the holes, 16 bytes a thread, four pieces under way.
-template <int PIECES>  // 16-byte pieces of a row
+template <int P>
 __global__ void __launch_bounds__(256) k_kv_move(dsh_kv_evict_t A, int most) {
-  const int h = blockIdx.y, count = A.work[h];
-  const int *hole = A.work + A.cache.n_heads + (int64_t)h * 2 * most, *mover = hole + most;
-  const int64_t rs = A.cache.row_stride * (A.cache.bf16 ? 2 : 4), hs = A.cache.head_stride * (A.cache.bf16 ? 2 : 4);
-  char *k = (char *)A.cache.k + h * hs, *v = (char *)A.cache.v + h * hs;
-  const int64_t total = (int64_t)count * 2 * PIECES, step = (int64_t)gridDim.x * 256;
-  for (int64_t x = blockIdx.x * 256 + threadIdx.x; x < total; x += 4 * step) {
-    u32x4 y[4];
-    char *to[4];
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      const int64_t i = x + u * step;
-      to[u] = nullptr;
-      if (i < total) {
-        const int r = (int)(i / (2 * PIECES)), piece = (int)(i - (int64_t)r * 2 * PIECES);
-        char *b = piece < PIECES ? k + 16 * piece : v + 16 * (piece - PIECES);
-        to[u] = b + hole[r] * rs;
-        y[u] = *(const u32x4 *)(b + mover[r] * rs);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 4; u++)
-      if (to[u]) *(u32x4 *)to[u] = y[u];
-  }
+  const int h = blockIdx.y;
+  const int *hole = A.work + A.cache.n_heads + (int64_t)h * 2 * most;
+  evict_move(A, h, A.work[h], hole, hole + most, P, blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
 }
 
 extern "C" {
@@ -301,18 +379,20 @@ size_t dsh_kv_evict_work(int n_heads, int n, int keep) { return (size_t)n_heads 
 hipError_t dsh_launch_kv_evict(const dsh_kv_evict_t *A, hipStream_t s) {
   const int most = evict_most(A->n, A->keep), G = A->cache.n_heads;
   const size_t lds = (size_t)(most + 1) * 2;  // 32 KB at most
+  const int pieces = A->cache.head_dim / (A->cache.bf16 ? 8 : 4);
+  // few rows are moved by the block that chose them
+  const int move = A->n <= 32 * ET && (int64_t)most * 32 * pieces <= EVICT_OWN ? pieces : 0;
   if (A->n <= 4 * ET)
-    k_kv_select<4><<<G, ET, lds, s>>>(*A, most);
+    k_kv_select<4><<<G, ET, lds, s>>>(*A, most, move);
   else if (A->n <= 8 * ET)
-    k_kv_select<8><<<G, ET, lds, s>>>(*A, most);
+    k_kv_select<8><<<G, ET, lds, s>>>(*A, most, move);
   else if (A->n <= 16 * ET)
-    k_kv_select<16><<<G, ET, lds, s>>>(*A, most);
+    k_kv_select<16><<<G, ET, lds, s>>>(*A, most, move);
   else if (A->n <= 32 * ET)
-    k_kv_select<32><<<G, ET, lds, s>>>(*A, most);
+    k_kv_select<32><<<G, ET, lds, s>>>(*A, most, move);
   else
     k_kv_select_long<<<G, ET, 0, s>>>(*A, most);
-  if (most == 0) return hipGetLastError();
-  const int pieces = A->cache.head_dim / (A->cache.bf16 ? 8 : 4);
+  if (most == 0 || move) return hipGetLastError();
   const int64_t want = ((int64_t)most * 2 * pieces + 1023) / 1024, cap = G < 2048 ? 2048 / G : 1;
   const dim3 g((unsigned)(want < cap ? want : cap), G);
 #define MV(N)                                      \
