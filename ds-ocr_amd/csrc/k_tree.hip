@@ -70,6 +70,9 @@ __device__ __forceinline__ bool tree_in_window(int p, int pos, int prefill_len, 
 //   f32 cache: v_mfma_f32_16x16x4, exact products and f32 sums. bf16 cache: v_mfma_f32_16x16x32_bf16, the f32 queries and
 //   weights in three bf16 parts each that add up to them exactly (24 bits), so that only the f32 sums round.
 #define ATT_SLACK 10.0f
+#ifndef STAGED_TILES
+#define STAGED_TILES 3
+#endif
 #define ATT_L2E 1.44269504088896340736f
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -80,6 +83,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 struct attend_plan {
   int tile_rows, pos_waves;  // 16-row tiles and shares of the positions in a block: a wave each
   int groups, splits;        // blocks per key head: groups of tile_rows tiles of rows, splits of the tiles of positions
+  int staged;                // k_tree_attend_rows
   int cache_tiles, tree_tiles, gap, skip, per;  // per: tiles of a split
   int grp;                                       // query heads per key head
   float inv_nodes;                               // 1 / n_nodes
@@ -444,6 +448,297 @@ __global__ void __launch_bounds__(64 * W, W == 4 && D <= 128 ? 2 : 1) k_tree_att
       put(nd, kh * P.grp + h, at0 + r, c + d, y, M, L, s_live[r]);
     }
   }
+}
+
+// The same where a key head has many rows: a block of W waves, a 16-row tile each, shares tiles of 32 positions through LDS.
+// With an f32 cache the products are bf16 ones as well, of three parts a number (split3) and without the three smallest of the
+// nine pairs (2^-21 of the product at most, all that is left out): 6 x 16 cycles where v_mfma_f32_16x16x4 takes 8 x 32, and the
+// parts are made once a block, when its threads write what they loaded to LDS. K lies there as rows of 16-byte pieces, V
+// transposed, 32 positions of a dimension in 64 bytes in the order of the summation index; both with the pieces' places
+// exclusive-ored so that the 16 lanes of a read hit all banks. Two blocks of four waves on a CU: one computes while the
+// other writes and waits.
+template <int D, bool BF>
+struct staged {
+  static constexpr int NL = BF ? 1 : 3, E = BF ? 8 : 4;  // parts; dimensions of a unit: 4 positions x E, 16 bytes a position
+  static constexpr int UNITS = 8 * (D / E);              // of K, and again of V
+  uint8_t k[NL][32 * D * 2], v[NL][D * 64];
+  uint32_t bad;  // positions with a V that is not finite (of a tile that some row does not see all of)
+  static __device__ __forceinline__ int k_at(int row, int piece) {
+    const int x = D % 128 == 0 ? row & 15 : (row >> 1) & 7;
+    return row * 2 * D + 16 * (piece ^ x);
+  }
+  static __device__ __forceinline__ int v_at(int d, int g) {
+    const int c = d >> 2;
+    return c * 256 + 16 * (((d & 3) * 4 + g) ^ (c & 15));
+  }
+};
+
+template <int D, bool BF, int W>
+__global__ void __launch_bounds__(64 * W, W == 4 && D <= 128 ? 2 : 1) k_tree_attend_rows(dsh_tree_attn_t A, attend_plan P) {
+  typedef staged<D, BF> stage;
+  constexpr int NL = stage::NL, E = stage::E, UNITS = stage::UNITS, U = (2 * UNITS + 64 * W - 1) / (64 * W), NS = D / 32;
+  __shared__ __attribute__((aligned(16))) stage S;
+  __shared__ tree_lds t;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, g = lane >> 4;
+  const int T = A.n_nodes, R = T * P.grp, kh = blockIdx.y, z = blockIdx.z, split = blockIdx.x, rt = wave;
+  const bool works = rt < P.tile_rows;  // the other waves only load
+  const int row = 16 * (z * P.tile_rows + rt) + i;
+  const int rr = min(row, R - 1), rh = (int)(((float)rr + 0.5f) * P.inv_nodes), node = rr - rh * T, head = kh * P.grp + rh;
+  const int tiles = P.cache_tiles - P.skip + P.tree_tiles, t0 = split * P.per, t1 = min(t0 + P.per, tiles);
+  const bool need = P.splits == 1 || A.scores || A.window > 0 || t1 > P.cache_tiles - P.skip;
+  const int parent = need ? tree_parent(A.parents, T) : -2;
+  struct where {
+    const char *k, *v;
+    int64_t rs;
+    int p0, end;
+    bool own;
+  };
+  const auto locate = [&](int tile) {
+    const int x = tile >= P.gap ? tile + P.skip : tile;
+    const bool own = x >= P.cache_tiles;
+    const dsh_kv_t &c = own ? A.tree : A.cache;
+    const int64_t h = kh * c.head_stride * (BF ? 2 : 4);
+    return where{(const char *)c.k + h, (const char *)c.v + h, c.row_stride * (BF ? 2 : 4), 32 * (own ? x - P.cache_tiles : x),
+                 own ? T : A.n_cache, own};
+  };
+  // the thread's units of a tile: unit u = tid + 64 W y, K's before V's; quad q of the positions, dimensions E c...
+  u32x4 st[U][4];
+  const auto load = [&](const where &w) {
+#pragma unroll
+    for (int y = 0; y < U; y++) {
+      const int u = tid + 64 * W * y;
+      if (2 * UNITS % (64 * W) && u >= 2 * UNITS) continue;
+      const int x = u < UNITS ? u : u - UNITS, q = x / (D / E), c = x - q * (D / E);
+      const char *p = (u < UNITS ? w.k : w.v) + 16 * c;
+#pragma unroll
+      for (int r = 0; r < 4; r++) st[y][r] = *(const u32x4 *)(p + min(w.p0 + 4 * q + r, w.end - 1) * w.rs);
+    }
+  };
+  const auto write = [&](bool part) {
+#pragma unroll
+    for (int y = 0; y < U; y++) {
+      const int u = tid + 64 * W * y;
+      if (2 * UNITS % (64 * W) && u >= 2 * UNITS) continue;
+      const bool is_v = u >= UNITS;
+      const int x = is_v ? u - UNITS : u, q = x / (D / E), c = x - q * (D / E);
+      if (part && is_v) {  // what is not finite becomes 0: see k_tree_attend
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          bool bad = false;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            if (BF) {
+              if ((st[y][r][e] & 0x7F80u) == 0x7F80u) bad = true, st[y][r][e] &= 0xFFFF0000u;
+              if ((st[y][r][e] & 0x7F800000u) == 0x7F800000u) bad = true, st[y][r][e] &= 0xFFFFu;
+            } else if ((st[y][r][e] & 0x7F800000u) == 0x7F800000u) {
+              bad = true;
+              st[y][r][e] = 0;
+            }
+          }
+          if (bad) atomicOr(&S.bad, 1u << (4 * q + r));
+        }
+      }
+      if (BF) {
+        if (!is_v) {
+#pragma unroll
+          for (int r = 0; r < 4; r++) *(u32x4 *)(S.k[0] + stage::k_at(4 * q + r, c)) = st[y][r];
+        } else {
+#pragma unroll
+          for (int d = 0; d < 8; d++) {
+            const uint32_t sel = d & 1 ? 0x07060302u : 0x05040100u;
+            uint2 w;
+            w.x = __builtin_amdgcn_perm(st[y][1][d >> 1], st[y][0][d >> 1], sel);
+            w.y = __builtin_amdgcn_perm(st[y][3][d >> 1], st[y][2][d >> 1], sel);
+            *(uint2 *)(S.v[0] + stage::v_at(8 * c + d, q & 3) + 8 * (q >> 2)) = w;
+          }
+        }
+      } else {
+        uint32_t a[3][4][4];  // part, position, dimension
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) split3(__uint_as_float(st[y][r][e]), a[0][r][e], a[1][r][e], a[2][r][e]);
+#pragma unroll
+        for (int n = 0; n < NL; n++) {
+          if (!is_v) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              uint2 w;
+              w.x = upper2(a[n][r][0], a[n][r][1]);
+              w.y = upper2(a[n][r][2], a[n][r][3]);
+              *(uint2 *)(S.k[n] + stage::k_at(4 * q + r, c >> 1) + 8 * (c & 1)) = w;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              uint2 w;
+              w.x = upper2(a[n][0][e], a[n][1][e]);
+              w.y = upper2(a[n][2][e], a[n][3][e]);
+              *(uint2 *)(S.v[n] + stage::v_at(4 * c + e, q & 3) + 8 * (q >> 2)) = w;
+            }
+          }
+        }
+      }
+    }
+  };
+  where nx = locate(t0);
+  load(nx);
+  // the wave's queries, in three parts
+  u32x4 qf[3][NS];
+  {
+    const float *p = A.q + node * A.q_stride + (int64_t)head * D + 8 * g;
+#pragma unroll
+    for (int x = 0; x < NS; x++) {
+      float y[8];
+      *(f32x4 *)y = *(const f32x4 *)(p + 32 * x);
+      *(f32x4 *)(y + 4) = *(const f32x4 *)(p + 32 * x + 4);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        uint32_t a[3], b[3];
+        split3(y[2 * e], a[0], a[1], a[2]);
+        split3(y[2 * e + 1], b[0], b[1], b[2]);
+#pragma unroll
+        for (int n = 0; n < 3; n++) qf[n][x][e] = upper2(a[n], b[n]);
+      }
+    }
+  }
+  if (tid == 0) S.bad = 0;
+  if (need) tree_ancestors(t, parent, T);
+  const u64 anc0 = need ? t.anc[node][0] : 0, anc1 = need ? t.anc[node][1] : 0;
+  const bool live = !need || (anc0 | anc1);
+  const int pos = A.n_cache + __popcll(anc0) + __popcll(anc1) - 1;
+  const int lo = A.window > 0 && pos >= A.prefill_len ? max(A.prefill_len, pos + 1 - A.window) : 0;
+  const float inf = __builtin_huge_valf();
+  float m = -inf, l = 0.0f, ml2 = 0.0f;
+  f32x4 o[D / 16];  // o[b][r]: dimension 16 b + 4 g + r of the lane's row
+#pragma unroll
+  for (int b = 0; b < D / 16; b++) o[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float *sc = A.scores ? A.scores + ((int64_t)head * T + node) * A.score_stride : nullptr;
+  const int lo_most = A.n_cache + T - A.window;
+#define MFMA(a, b, c) \
+  __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0)
+  __syncthreads();
+  for (int tile = t0; tile < t1; tile++) {
+    const bool own = nx.own;
+    const int p0 = nx.p0, end = nx.end;
+    const bool part = own || p0 + 32 > end || (A.window > 0 && p0 + 32 > A.prefill_len && p0 < lo_most);
+    write(part);
+    __syncthreads();
+    nx = locate(min(tile + 1, tiles - 1));
+    load(nx);
+    if (works) {
+      float s[8];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        f32x4 a[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int x = 0; x < NS; x++) {
+          u32x4 f[NL];
+#pragma unroll
+          for (int n = 0; n < NL; n++) f[n] = *(const u32x4 *)(S.k[n] + stage::k_at(16 * h + i, 4 * x + g));
+#pragma unroll
+          for (int sum = 2; sum >= 0; sum--)  // the small products first
+#pragma unroll
+            for (int n = 0; n < NL; n++)
+              if (sum - n >= 0 && sum - n < 3) a[x & 1] = MFMA(f[n], qf[sum - n][x], a[x & 1]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[4 * h + r] = (a[0][r] + a[1][r]) * A.scale;
+      }
+      if (part) {
+        const uint32_t bad = S.bad;
+        bool poison = false;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const int at = 16 * (k >> 2) + 4 * g + (k & 3), j = p0 + at;
+          bool see = live && j < end;
+          int p = j;
+          if (own) {
+            const int a = min(j, DSH_TREE_MAX - 1);
+            see = see && (((a < 64 ? anc0 >> a : anc1 >> (a - 64)) & 1) != 0);
+            if (A.window > 0) p = A.n_cache + tree_depth(t.anc[a]);
+          }
+          see = see && (p < A.prefill_len || p >= lo);
+          s[k] = see ? s[k] : -inf;
+          poison |= see && ((bad >> at) & 1);
+        }
+        if (__any(poison)) {
+          int y = poison;
+          y |= __shfl_xor(y, 16);
+          y |= __shfl_xor(y, 32);
+          if (y)
+#pragma unroll
+            for (int b = 0; b < D / 16; b++) o[b] += __builtin_nanf("");
+        }
+      }
+      if (sc && row < R) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const int j = p0 + 16 * (k >> 2) + 4 * g + (k & 3);
+          if (j < end) sc[own ? (int64_t)A.n_cache + j : j] = live ? s[k] : -inf;
+        }
+      }
+      float mx = s[0];
+#pragma unroll
+      for (int k = 1; k < 8; k++) mx = fmaxf(mx, s[k]);
+      if (__any(mx > m + ATT_SLACK)) {
+        mx = fmaxf(mx, m);
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float f = mx == m ? 1.0f : att_exp(m - mx);
+        m = mx;
+        ml2 = m == -inf ? 0.0f : m * ATT_L2E;
+        l *= f;
+#pragma unroll
+        for (int b = 0; b < D / 16; b++) o[b] *= f;
+      }
+      u32x4 pf[3];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        uint32_t a[3], b[3];
+#pragma unroll
+        for (int k = 2 * e; k < 2 * e + 2; k++) {
+          s[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], ATT_L2E, -ml2));
+          l += s[k];
+        }
+        split3(s[2 * e], a[0], a[1], a[2]);
+        split3(s[2 * e + 1], b[0], b[1], b[2]);
+#pragma unroll
+        for (int n = 0; n < 3; n++) pf[n][e] = upper2(a[n], b[n]);
+      }
+#pragma unroll
+      for (int b = 0; b < D / 16; b++) {
+        u32x4 f[NL];
+#pragma unroll
+        for (int n = 0; n < NL; n++) f[n] = *(const u32x4 *)(S.v[n] + stage::v_at(16 * b + i, g));
+#pragma unroll
+        for (int sum = 2; sum >= 0; sum--)
+#pragma unroll
+          for (int n = 0; n < NL; n++)
+            if (sum - n >= 0 && sum - n < 3) o[b] = MFMA(f[n], pf[sum - n], o[b]);
+      }
+    }
+    __syncthreads();
+    if (part && tid == 0) S.bad = 0;  // before the next write's, which a barrier follows
+    if (part) __syncthreads();
+  }
+#undef MFMA
+  if (!works || row >= R) return;
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (P.splits > 1) {
+    const int64_t at = (((int64_t)kh * P.groups + z) * P.splits + split) * 16 * P.tile_rows + 16 * rt + i;
+#pragma unroll
+    for (int b = 0; b < D / 16; b++) *(f32x4 *)(P.part + at * D + 16 * b + 4 * g) = o[b];
+    if (g == 0) *(f32x2 *)(P.ml + 2 * at) = f32x2{m, l};
+    return;
+  }
+  const bool none = !live || l == 0.0f;
+#pragma unroll
+  for (int b = 0; b < D / 16; b++)
+    *(f32x4 *)(A.out + node * A.out_stride + (int64_t)head * D + 16 * b + 4 * g) =
+        none ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o[b] * (1.0f / l);
+  if (A.lse && g == 0) A.lse[(int64_t)head * T + node] = none ? -inf : m + logf(l);
 }
 
 // The splits of one row put together, in their order: a block of D threads per row, the maxima and sums by its first wave.
@@ -874,12 +1169,13 @@ extern "C" {
 static attend_plan attend_cut(const dsh_tree_attn_t *A) {
   attend_plan P;
   memset(&P, 0, sizeof P);
-  const int AT = A->cache.bf16 ? 32 : 16, G = A->cache.n_heads;
+  const int G = A->cache.n_heads, D = A->cache.head_dim;
   const int64_t rows = (int64_t)A->n_nodes * (A->n_heads / G), row_tiles = (rows + 15) / 16;
-  const int most = A->cache.head_dim <= 128 ? 8 : 4;
+  P.staged = row_tiles >= STAGED_TILES && (A->cache.bf16 || D <= 128);
+  const int AT = A->cache.bf16 || P.staged ? 32 : 16, most = D <= 128 ? 8 : 4;
   P.groups = (int)((row_tiles + most - 1) / most);
   P.tile_rows = (int)((row_tiles + P.groups - 1) / P.groups);
-  P.pos_waves = P.tile_rows == 1 ? 4 : P.tile_rows == 2 ? 2 : 1;
+  P.pos_waves = P.staged || P.tile_rows > 2 ? 1 : P.tile_rows == 1 ? 4 : 2;
   P.cache_tiles = (int)(((int64_t)A->n_cache + AT - 1) / AT);
   P.tree_tiles = (A->n_nodes + AT - 1) / AT;
   P.gap = P.cache_tiles;
@@ -926,7 +1222,14 @@ hipError_t dsh_launch_tree_attention(const dsh_tree_attn_t *A, float *work, hipS
   const size_t lds = P.pos_waves > 1 ? (size_t)W * 16 * ((D < 128 ? D : 128) + 4) * 4 : 0;
 #define CASE(D, BF)                                                                   \
   case D:                                                                             \
-    if (W <= 4)                                                                       \
+    if (P.staged) {                                                                   \
+      if constexpr (BF || D <= 128) {                                                 \
+        if (D > 128 || P.tile_rows <= 4)                                              \
+          k_tree_attend_rows<D, BF, 4><<<grid, 256, 0, s>>>(*A, P);                   \
+        else if constexpr (D <= 128)                                                  \
+          k_tree_attend_rows<D, BF, 8><<<grid, 512, 0, s>>>(*A, P);                   \
+      }                                                                               \
+    } else if (W <= 4)                                                                \
       k_tree_attend<D, BF, 4><<<grid, 64 * W, lds, s>>>(*A, P);                       \
     else                                                                              \
       k_tree_attend<D, BF, 8><<<grid, 64 * W, lds, s>>>(*A, P);                       \
