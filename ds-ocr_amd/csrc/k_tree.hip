@@ -450,38 +450,41 @@ __global__ void __launch_bounds__(64 * W, W == 4 && D <= 128 ? 2 : 1) k_tree_att
   }
 }
 
-// The same where a key head has many rows: a block of W waves, a 16-row tile each, shares tiles of 32 positions through LDS.
-// With an f32 cache the products are bf16 ones as well, of three parts a number (split3) and without the three smallest of the
-// nine pairs (2^-21 of the product at most, all that is left out): 6 x 16 cycles where v_mfma_f32_16x16x4 takes 8 x 32, and the
-// parts are made once a block, when its threads write what they loaded to LDS. K lies there as rows of 16-byte pieces, V
+// The same where a key head has many rows: a block of eight waves, up to eight 16-row tiles, shares tiles of 32 positions through
+// LDS. With an f32 cache the products are bf16 ones as well, of three parts a number (split3) and without the three smallest
+// of the nine pairs (2^-21 of the product at most, all that is left out): 6 x 16 cycles where v_mfma_f32_16x16x4 takes 8 x 32,
+// and the parts are made once a block, when what was loaded is written to LDS. K lies there as rows of 16-byte pieces, V
 // transposed, 32 positions of a dimension in 64 bytes in the order of the summation index; both with the pieces' places
-// exclusive-ored so that the 16 lanes of a read hit all banks. Two blocks of four waves on a CU: one computes while the
-// other writes and waits.
+// exclusive-ored so that the 16 lanes of a read or write meet all banks. The last SW waves bring the next tile into the other
+// half of the LDS while the others compute, one of each kind to a SIMD, so that the vector units' splitting and the matrix
+// units' products go on at once; where there are rows for all eight (SW = 8), each does both, half of them in the other order.
 template <int D, bool BF>
 struct staged {
   static constexpr int NL = BF ? 1 : 3, E = BF ? 8 : 4;  // parts; dimensions of a unit: 4 positions x E, 16 bytes a position
   static constexpr int UNITS = 8 * (D / E);              // of K, and again of V
   uint8_t k[NL][32 * D * 2], v[NL][D * 64];
-  uint32_t bad;  // positions with a V that is not finite (of a tile that some row does not see all of)
   static __device__ __forceinline__ int k_at(int row, int piece) {
     const int x = D % 128 == 0 ? row & 15 : (row >> 1) & 7;
     return row * 2 * D + 16 * (piece ^ x);
   }
   static __device__ __forceinline__ int v_at(int d, int g) {
     const int c = d >> 2;
-    return c * 256 + 16 * (((d & 3) * 4 + g) ^ (c & 15));
+    return c * 256 + 16 * (((d & 3) * 4 + g) ^ ((c ^ (c >> 4)) & 15));
   }
 };
 
-template <int D, bool BF, int W>
-__global__ void __launch_bounds__(64 * W, W == 4 && D <= 128 ? 2 : 1) k_tree_attend_rows(dsh_tree_attn_t A, attend_plan P) {
+template <int D, bool BF, int SW>
+__global__ void __launch_bounds__(512) k_tree_attend_rows(dsh_tree_attn_t A, attend_plan P) {
   typedef staged<D, BF> stage;
-  constexpr int NL = stage::NL, E = stage::E, UNITS = stage::UNITS, U = (2 * UNITS + 64 * W - 1) / (64 * W), NS = D / 32;
-  __shared__ __attribute__((aligned(16))) stage S;
+  constexpr int NL = stage::NL, E = stage::E, UNITS = stage::UNITS, SN = 64 * SW, U = (2 * UNITS + SN - 1) / SN, NS = D / 32;
+  constexpr int AHEAD = U * (BF ? 3 : 2) <= 8 ? BF ? 3 : 2 : 1;  // tiles on their way, in registers
+  __shared__ __attribute__((aligned(16))) stage S[2];
+  __shared__ uint32_t s_bad[3];  // by the tile: positions with a V that is not finite (where some row does not see all of it)
   __shared__ tree_lds t;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, g = lane >> 4;
   const int T = A.n_nodes, R = T * P.grp, kh = blockIdx.y, z = blockIdx.z, split = blockIdx.x, rt = wave;
-  const bool works = rt < P.tile_rows;  // the other waves only load
+  const bool works = rt < P.tile_rows, stager = wave >= 8 - SW;
+  const int sid = tid - 64 * (8 - SW);
   const int row = 16 * (z * P.tile_rows + rt) + i;
   const int rr = min(row, R - 1), rh = (int)(((float)rr + 0.5f) * P.inv_nodes), node = rr - rh * T, head = kh * P.grp + rh;
   const int tiles = P.cache_tiles - P.skip + P.tree_tiles, t0 = split * P.per, t1 = min(t0 + P.per, tiles);
@@ -501,24 +504,23 @@ __global__ void __launch_bounds__(64 * W, W == 4 && D <= 128 ? 2 : 1) k_tree_att
     return where{(const char *)c.k + h, (const char *)c.v + h, c.row_stride * (BF ? 2 : 4), 32 * (own ? x - P.cache_tiles : x),
                  own ? T : A.n_cache, own};
   };
-  // the thread's units of a tile: unit u = tid + 64 W y, K's before V's; quad q of the positions, dimensions E c...
-  u32x4 st[U][4];
-  const auto load = [&](const where &w) {
+  // the thread's units of a tile: unit u = sid + SN y, K's before V's; quad q of the positions, dimensions E c...
+  const auto load = [&](u32x4 (*st)[4], const where &w) {
 #pragma unroll
     for (int y = 0; y < U; y++) {
-      const int u = tid + 64 * W * y;
-      if (2 * UNITS % (64 * W) && u >= 2 * UNITS) continue;
+      const int u = sid + SN * y;
+      if (2 * UNITS % SN && u >= 2 * UNITS) continue;
       const int x = u < UNITS ? u : u - UNITS, q = x / (D / E), c = x - q * (D / E);
       const char *p = (u < UNITS ? w.k : w.v) + 16 * c;
 #pragma unroll
       for (int r = 0; r < 4; r++) st[y][r] = *(const u32x4 *)(p + min(w.p0 + 4 * q + r, w.end - 1) * w.rs);
     }
   };
-  const auto write = [&](bool part) {
+  const auto write = [&](u32x4 (*st)[4], stage &S, bool part, uint32_t *bad_word) {
 #pragma unroll
     for (int y = 0; y < U; y++) {
-      const int u = tid + 64 * W * y;
-      if (2 * UNITS % (64 * W) && u >= 2 * UNITS) continue;
+      const int u = sid + SN * y;
+      if (2 * UNITS % SN && u >= 2 * UNITS) continue;
       const bool is_v = u >= UNITS;
       const int x = is_v ? u - UNITS : u, q = x / (D / E), c = x - q * (D / E);
       if (part && is_v) {  // what is not finite becomes 0: see k_tree_attend
@@ -535,7 +537,7 @@ __global__ void __launch_bounds__(64 * W, W == 4 && D <= 128 ? 2 : 1) k_tree_att
               st[y][r][e] = 0;
             }
           }
-          if (bad) atomicOr(&S.bad, 1u << (4 * q + r));
+          if (bad) atomicOr(bad_word, 1u << (4 * q + r));
         }
       }
       if (BF) {
@@ -581,8 +583,39 @@ __global__ void __launch_bounds__(64 * W, W == 4 && D <= 128 ? 2 : 1) k_tree_att
       }
     }
   };
-  where nx = locate(t0);
-  load(nx);
+  const int lo_most = A.n_cache + T - A.window;
+  // whether some row may not see all of a tile
+  const auto partial = [&](const where &w) {
+    return w.own || w.p0 + 32 > w.end || (A.window > 0 && w.p0 + 32 > A.prefill_len && w.p0 < lo_most);
+  };
+  u32x4 ahead[AHEAD][U][4];
+  if (stager) {
+#pragma unroll
+    for (int a = 0; a < AHEAD; a++) load(ahead[a], locate(min(t0 + a, tiles - 1)));
+  }
+  // Tile t0 + n (n % AHEAD == a) to its half of the LDS, and the loads of the tile AHEAD after it.
+  const auto bring = [&](int n, u32x4 (*st)[4]) {
+    const where w = locate(t0 + n);
+    write(st, S[n & 1], partial(w), &s_bad[n % 3]);
+    if (sid == 0) s_bad[(n + 1) % 3] = 0;  // read two tiles ago
+    load(st, locate(min(t0 + n + AHEAD, tiles - 1)));
+  };
+  if (tid < 3) s_bad[tid] = 0;
+  if (need) tree_ancestors(t, parent, T);
+  const int count = t1 - t0;
+  if (SW < 8 && stager) {
+    __syncthreads();
+    bring(0, ahead[0]);
+    __syncthreads();
+    for (int n0 = 0; n0 < count; n0 += AHEAD)
+#pragma unroll
+      for (int a = 0; a < AHEAD; a++) {
+        if (n0 + a >= count) break;
+        if (n0 + a + 1 < count) bring(n0 + a + 1, ahead[(a + 1) % AHEAD]);
+        __syncthreads();
+      }
+    return;
+  }
   // the wave's queries, in three parts
   u32x4 qf[3][NS];
   {
@@ -602,8 +635,6 @@ __global__ void __launch_bounds__(64 * W, W == 4 && D <= 128 ? 2 : 1) k_tree_att
       }
     }
   }
-  if (tid == 0) S.bad = 0;
-  if (need) tree_ancestors(t, parent, T);
   const u64 anc0 = need ? t.anc[node][0] : 0, anc1 = need ? t.anc[node][1] : 0;
   const bool live = !need || (anc0 | anc1);
   const int pos = A.n_cache + __popcll(anc0) + __popcll(anc1) - 1;
@@ -614,113 +645,125 @@ __global__ void __launch_bounds__(64 * W, W == 4 && D <= 128 ? 2 : 1) k_tree_att
 #pragma unroll
   for (int b = 0; b < D / 16; b++) o[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float *sc = A.scores ? A.scores + ((int64_t)head * T + node) * A.score_stride : nullptr;
-  const int lo_most = A.n_cache + T - A.window;
 #define MFMA(a, b, c) \
   __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0)
-  __syncthreads();
-  for (int tile = t0; tile < t1; tile++) {
-    const bool own = nx.own;
-    const int p0 = nx.p0, end = nx.end;
-    const bool part = own || p0 + 32 > end || (A.window > 0 && p0 + 32 > A.prefill_len && p0 < lo_most);
-    write(part);
-    __syncthreads();
-    nx = locate(min(tile + 1, tiles - 1));
-    load(nx);
-    if (works) {
-      float s[8];
+  const auto compute = [&](int tile) {
+    const where now = locate(t0 + tile);
+    const bool own = now.own, part = partial(now);
+    const int p0 = now.p0, end = now.end;
+    const stage &C = S[tile & 1];
+    float s[8];
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        f32x4 a[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    for (int h = 0; h < 2; h++) {
+      f32x4 a[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-        for (int x = 0; x < NS; x++) {
-          u32x4 f[NL];
-#pragma unroll
-          for (int n = 0; n < NL; n++) f[n] = *(const u32x4 *)(S.k[n] + stage::k_at(16 * h + i, 4 * x + g));
-#pragma unroll
-          for (int sum = 2; sum >= 0; sum--)  // the small products first
-#pragma unroll
-            for (int n = 0; n < NL; n++)
-              if (sum - n >= 0 && sum - n < 3) a[x & 1] = MFMA(f[n], qf[sum - n][x], a[x & 1]);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; r++) s[4 * h + r] = (a[0][r] + a[1][r]) * A.scale;
-      }
-      if (part) {
-        const uint32_t bad = S.bad;
-        bool poison = false;
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const int at = 16 * (k >> 2) + 4 * g + (k & 3), j = p0 + at;
-          bool see = live && j < end;
-          int p = j;
-          if (own) {
-            const int a = min(j, DSH_TREE_MAX - 1);
-            see = see && (((a < 64 ? anc0 >> a : anc1 >> (a - 64)) & 1) != 0);
-            if (A.window > 0) p = A.n_cache + tree_depth(t.anc[a]);
-          }
-          see = see && (p < A.prefill_len || p >= lo);
-          s[k] = see ? s[k] : -inf;
-          poison |= see && ((bad >> at) & 1);
-        }
-        if (__any(poison)) {
-          int y = poison;
-          y |= __shfl_xor(y, 16);
-          y |= __shfl_xor(y, 32);
-          if (y)
-#pragma unroll
-            for (int b = 0; b < D / 16; b++) o[b] += __builtin_nanf("");
-        }
-      }
-      if (sc && row < R) {
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const int j = p0 + 16 * (k >> 2) + 4 * g + (k & 3);
-          if (j < end) sc[own ? (int64_t)A.n_cache + j : j] = live ? s[k] : -inf;
-        }
-      }
-      float mx = s[0];
-#pragma unroll
-      for (int k = 1; k < 8; k++) mx = fmaxf(mx, s[k]);
-      if (__any(mx > m + ATT_SLACK)) {
-        mx = fmaxf(mx, m);
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float f = mx == m ? 1.0f : att_exp(m - mx);
-        m = mx;
-        ml2 = m == -inf ? 0.0f : m * ATT_L2E;
-        l *= f;
-#pragma unroll
-        for (int b = 0; b < D / 16; b++) o[b] *= f;
-      }
-      u32x4 pf[3];
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        uint32_t a[3], b[3];
-#pragma unroll
-        for (int k = 2 * e; k < 2 * e + 2; k++) {
-          s[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], ATT_L2E, -ml2));
-          l += s[k];
-        }
-        split3(s[2 * e], a[0], a[1], a[2]);
-        split3(s[2 * e + 1], b[0], b[1], b[2]);
-#pragma unroll
-        for (int n = 0; n < 3; n++) pf[n][e] = upper2(a[n], b[n]);
-      }
-#pragma unroll
-      for (int b = 0; b < D / 16; b++) {
+      for (int x = 0; x < NS; x++) {
         u32x4 f[NL];
 #pragma unroll
-        for (int n = 0; n < NL; n++) f[n] = *(const u32x4 *)(S.v[n] + stage::v_at(16 * b + i, g));
+        for (int n = 0; n < NL; n++) f[n] = *(const u32x4 *)(C.k[n] + stage::k_at(16 * h + i, 4 * x + g));
 #pragma unroll
-        for (int sum = 2; sum >= 0; sum--)
+        for (int sum = 2; sum >= 0; sum--)  // the small products first
 #pragma unroll
           for (int n = 0; n < NL; n++)
-            if (sum - n >= 0 && sum - n < 3) o[b] = MFMA(f[n], pf[sum - n], o[b]);
+            if (sum - n >= 0 && sum - n < 3) a[x & 1] = MFMA(f[n], qf[sum - n][x], a[x & 1]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; r++) s[4 * h + r] = (a[0][r] + a[1][r]) * A.scale;
+    }
+    if (part) {
+      const uint32_t bad = s_bad[tile % 3];
+      bool poison = false;
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const int at = 16 * (k >> 2) + 4 * g + (k & 3), j = p0 + at;
+        bool see = live && j < end;
+        int p = j;
+        if (own) {
+          const int a = min(j, DSH_TREE_MAX - 1);
+          see = see && (((a < 64 ? anc0 >> a : anc1 >> (a - 64)) & 1) != 0);
+          if (A.window > 0) p = A.n_cache + tree_depth(t.anc[a]);
+        }
+        see = see && (p < A.prefill_len || p >= lo);
+        s[k] = see ? s[k] : -inf;
+        poison |= see && ((bad >> at) & 1);
+      }
+      if (__any(poison)) {
+        int y = poison;
+        y |= __shfl_xor(y, 16);
+        y |= __shfl_xor(y, 32);
+        if (y)
+#pragma unroll
+          for (int b = 0; b < D / 16; b++) o[b] += __builtin_nanf("");
       }
     }
+    if (sc && row < R) {
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const int j = p0 + 16 * (k >> 2) + 4 * g + (k & 3);
+        if (j < end) sc[own ? (int64_t)A.n_cache + j : j] = live ? s[k] : -inf;
+      }
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int k = 1; k < 8; k++) mx = fmaxf(mx, s[k]);
+    if (__any(mx > m + ATT_SLACK)) {
+      mx = fmaxf(mx, m);
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float f = mx == m ? 1.0f : att_exp(m - mx);
+      m = mx;
+      ml2 = m == -inf ? 0.0f : m * ATT_L2E;
+      l *= f;
+#pragma unroll
+      for (int b = 0; b < D / 16; b++) o[b] *= f;
+    }
+    u32x4 pf[3];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      uint32_t a[3], b[3];
+#pragma unroll
+      for (int k = 2 * e; k < 2 * e + 2; k++) {
+        s[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], ATT_L2E, -ml2));
+        l += s[k];
+      }
+      split3(s[2 * e], a[0], a[1], a[2]);
+      split3(s[2 * e + 1], b[0], b[1], b[2]);
+#pragma unroll
+      for (int n = 0; n < 3; n++) pf[n][e] = upper2(a[n], b[n]);
+    }
+#pragma unroll
+    for (int b = 0; b < D / 16; b++) {
+      u32x4 f[NL];
+#pragma unroll
+      for (int n = 0; n < NL; n++) f[n] = *(const u32x4 *)(C.v[n] + stage::v_at(16 * b + i, g));
+#pragma unroll
+      for (int sum = 2; sum >= 0; sum--)
+#pragma unroll
+        for (int n = 0; n < NL; n++)
+          if (sum - n >= 0 && sum - n < 3) o[b] = MFMA(f[n], pf[sum - n], o[b]);
+    }
+  };
+  // one barrier a tile: tile n is read while tile n + 1 is written to the other half
+  __syncthreads();
+  if (SW == 8) {
+    bring(0, ahead[0]);
     __syncthreads();
-    if (part && tid == 0) S.bad = 0;  // before the next write's, which a barrier follows
-    if (part) __syncthreads();
+    for (int n0 = 0; n0 < count; n0 += AHEAD)
+#pragma unroll
+      for (int a = 0; a < AHEAD; a++) {
+        const int n = n0 + a;
+        if (n >= count) break;
+        if (n + 1 < count && wave >= 4) bring(n + 1, ahead[(a + 1) % AHEAD]);
+        if (works) compute(n);
+        if (n + 1 < count && wave < 4) bring(n + 1, ahead[(a + 1) % AHEAD]);
+        __syncthreads();
+      }
+  } else {
+    __syncthreads();
+    for (int n = 0; n < count; n++) {
+      if (works) compute(n);
+      __syncthreads();
+    }
   }
 #undef MFMA
   if (!works || row >= R) return;
@@ -741,41 +784,67 @@ __global__ void __launch_bounds__(64 * W, W == 4 && D <= 128 ? 2 : 1) k_tree_att
   if (A.lse && g == 0) A.lse[(int64_t)head * T + node] = none ? -inf : m + logf(l);
 }
 
-// The splits of one row put together, in their order: a block of D threads per row, the maxima and sums by its first wave.
+// The splits of one row put together: a block per row, D / 4 threads to a split, 1024 / D splits at a time in their order.
 template <int D>
 __global__ void __launch_bounds__(256) k_tree_join(dsh_tree_attn_t A, attend_plan P) {
+  constexpr int L = D / 4, N = 256 / L;
   __shared__ tree_lds t;
   __shared__ float s_f[1024], s_inv;
+  __shared__ __attribute__((aligned(16))) float s_o[N][D];
   const int T = A.n_nodes, row = blockIdx.x, kh = blockIdx.y, rh = (int)(((float)row + 0.5f) * P.inv_nodes);
   const int node = row - rh * T, head = kh * P.grp + rh;
   const int z = (row >> 4) / P.tile_rows, in = row - z * 16 * P.tile_rows, stride = 16 * P.tile_rows;
   const int64_t at = ((int64_t)kh * P.groups + z) * P.splits * stride + in;
-  tree_ancestors(t, tree_parent(A.parents, T), T);
+  const int parent = tree_parent(A.parents, T);
+  const int x = threadIdx.x / L, d = 4 * (threadIdx.x - x * L);
+  const float *p = P.part + at * D + d;
+  // a thread's first splits are on their way while the factors are made
+  constexpr int AHEAD = 8;
+  f32x4 v[AHEAD];
+#pragma unroll
+  for (int u = 0; u < AHEAD; u++) v[u] = *(const f32x4 *)(p + (int64_t)min(x + N * u, P.splits - 1) * stride * D);
+  float mk = -__builtin_huge_valf(), lk = 0.0f;
+  if ((int)threadIdx.x < 64 && (int)threadIdx.x < P.splits) {
+    mk = P.ml[2 * (at + (int64_t)threadIdx.x * stride)];
+    lk = P.ml[2 * (at + (int64_t)threadIdx.x * stride) + 1];
+  }
+  tree_ancestors(t, parent, T);
   const bool live = t.anc[node][0] | t.anc[node][1];
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
-    float M = -__builtin_huge_valf(), L = 0.0f;
-    for (int k = lane; k < P.splits; k += 64) M = fmaxf(M, P.ml[2 * (at + (int64_t)k * stride)]);
+    float M = mk;
+    for (int k = lane + 64; k < P.splits; k += 64) M = fmaxf(M, P.ml[2 * (at + (int64_t)k * stride)]);
     M = dsh_wave_max(M);
-    for (int k = lane; k < P.splits; k += 64) {
-      const float mk = P.ml[2 * (at + (int64_t)k * stride)], f = mk == M ? 1.0f : att_exp(mk - M);
+    float f = mk == M ? 1.0f : att_exp(mk - M), sum = f * lk;
+    s_f[lane] = f;
+    for (int k = lane + 64; k < P.splits; k += 64) {
+      const float m = P.ml[2 * (at + (int64_t)k * stride)];
+      f = m == M ? 1.0f : att_exp(m - M);
       s_f[k] = f;
-      L += f * P.ml[2 * (at + (int64_t)k * stride) + 1];
+      sum += f * P.ml[2 * (at + (int64_t)k * stride) + 1];
     }
-    L = dsh_wave_sum(L);
-    const bool none = !live || L == 0.0f;
+    sum = dsh_wave_sum(sum);
+    const bool none = !live || sum == 0.0f;
     if (lane == 0) {
-      s_inv = none ? 0.0f : 1.0f / L;
-      if (A.lse) A.lse[(int64_t)head * T + node] = none ? -__builtin_huge_valf() : M + logf(L);
+      s_inv = none ? 0.0f : 1.0f / sum;
+      if (A.lse) A.lse[(int64_t)head * T + node] = none ? -__builtin_huge_valf() : M + logf(sum);
     }
   }
   __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= D) return;
-  float a = 0.0f;
-  const float *p = P.part + at * D + d;
-  for (int k = 0; k < P.splits; k++) a = __builtin_fmaf(s_f[k], p[(int64_t)k * stride * D], a);
-  A.out[node * A.out_stride + (int64_t)head * D + d] = s_inv == 0.0f ? 0.0f : a * s_inv;
+  f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (x < N) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++)
+      if (x + N * u < P.splits) a += s_f[x + N * u] * v[u];
+    for (int k = x + N * AHEAD; k < P.splits; k += N) a += s_f[k] * *(const f32x4 *)(p + (int64_t)k * stride * D);
+    *(f32x4 *)(s_o[x] + d) = a;
+  }
+  __syncthreads();
+  if ((int)threadIdx.x >= D) return;
+  float y = 0.0f;
+#pragma unroll
+  for (int k = 0; k < N; k++) y += s_o[k][threadIdx.x];
+  A.out[node * A.out_stride + (int64_t)head * D + threadIdx.x] = s_inv == 0.0f ? 0.0f : y * s_inv;
 }
 
 // ---------------------------------------------------------------------------- verification
@@ -1172,7 +1241,7 @@ static attend_plan attend_cut(const dsh_tree_attn_t *A) {
   const int G = A->cache.n_heads, D = A->cache.head_dim;
   const int64_t rows = (int64_t)A->n_nodes * (A->n_heads / G), row_tiles = (rows + 15) / 16;
   P.staged = row_tiles >= STAGED_TILES && (A->cache.bf16 || D <= 128);
-  const int AT = A->cache.bf16 || P.staged ? 32 : 16, most = D <= 128 ? 8 : 4;
+  const int AT = A->cache.bf16 || P.staged ? 32 : 16, most = P.staged || D <= 128 ? 8 : 4;
   P.groups = (int)((row_tiles + most - 1) / most);
   P.tile_rows = (int)((row_tiles + P.groups - 1) / P.groups);
   P.pos_waves = P.staged || P.tile_rows > 2 ? 1 : P.tile_rows == 1 ? 4 : 2;
@@ -1190,7 +1259,7 @@ static attend_plan attend_cut(const dsh_tree_attn_t *A) {
   }
   const int64_t tiles = (int64_t)P.cache_tiles - P.skip + P.tree_tiles;
   // two blocks of four waves fit a CU, one of more
-  const int64_t want = (P.tile_rows * P.pos_waves <= 4 ? 512 : 256) / ((int64_t)G * P.groups);
+  const int64_t want = (!P.staged && P.tile_rows * P.pos_waves <= 4 ? 512 : 256) / ((int64_t)G * P.groups);
   // up to four tiles a wave cost less than a second kernel that joins splits
   int64_t splits = (tiles + P.pos_waves - 1) / P.pos_waves;
   if (splits <= 4) splits = 1;
@@ -1224,9 +1293,11 @@ hipError_t dsh_launch_tree_attention(const dsh_tree_attn_t *A, float *work, hipS
   case D:                                                                             \
     if (P.staged) {                                                                   \
       if constexpr (BF || D <= 128) {                                                 \
-        if (D > 128 || P.tile_rows <= 4)                                              \
-          k_tree_attend_rows<D, BF, 4><<<grid, 256, 0, s>>>(*A, P);                   \
-        else if constexpr (D <= 128)                                                  \
+        if (P.tile_rows <= 4)                                                         \
+          k_tree_attend_rows<D, BF, 4><<<grid, 512, 0, s>>>(*A, P);                   \
+        else if (P.tile_rows <= 6)                                                    \
+          k_tree_attend_rows<D, BF, 2><<<grid, 512, 0, s>>>(*A, P);                   \
+        else                                                                          \
           k_tree_attend_rows<D, BF, 8><<<grid, 512, 0, s>>>(*A, P);                   \
       }                                                                               \
     } else if (W <= 4)                                                                \
