@@ -506,14 +506,24 @@ __global__ void __launch_bounds__(512) k_tree_attend_rows(dsh_tree_attn_t A, att
   };
   // the thread's units of a tile: unit u = sid + SN y, K's before V's; quad q of the positions, dimensions E c...
   const auto load = [&](u32x4 (*st)[4], const where &w) {
+    const int64_t r1 = w.rs, r3 = 3 * w.rs;
+    const bool whole = w.p0 + 32 <= w.end;
 #pragma unroll
     for (int y = 0; y < U; y++) {
       const int u = sid + SN * y;
       if (2 * UNITS % SN && u >= 2 * UNITS) continue;
       const int x = u < UNITS ? u : u - UNITS, q = x / (D / E), c = x - q * (D / E);
-      const char *p = (u < UNITS ? w.k : w.v) + 16 * c;
+      const char *b = (u < UNITS ? w.k : w.v) + 16 * c;
+      if (whole) {
+        const char *p = b + w.p0 * w.rs + 4 * q * w.rs;
+        st[y][0] = *(const u32x4 *)p;
+        st[y][1] = *(const u32x4 *)(p + r1);
+        st[y][2] = *(const u32x4 *)(p + 2 * r1);
+        st[y][3] = *(const u32x4 *)(p + r3);
+      } else {
 #pragma unroll
-      for (int r = 0; r < 4; r++) st[y][r] = *(const u32x4 *)(p + min(w.p0 + 4 * q + r, w.end - 1) * w.rs);
+        for (int r = 0; r < 4; r++) st[y][r] = *(const u32x4 *)(b + min(w.p0 + 4 * q + r, w.end - 1) * w.rs);
+      }
     }
   };
   const auto write = [&](u32x4 (*st)[4], stage &S, bool part, uint32_t *bad_word) {
@@ -653,23 +663,41 @@ __global__ void __launch_bounds__(512) k_tree_attend_rows(dsh_tree_attn_t A, att
     const int p0 = now.p0, end = now.end;
     const stage &C = S[tile & 1];
     float s[8];
+    constexpr bool EARLY = BF && D <= 128;  // all of a tile's reads from LDS ahead of their use, where registers allow
+    u32x4 f[2][EARLY ? NS : 1][NL], fv[EARLY ? D / 16 : 1][NL];
+    const auto read_k = [&](int h, int x) {
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      f32x4 a[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+      for (int n = 0; n < NL; n++) f[h][EARLY ? x : 0][n] = *(const u32x4 *)(C.k[n] + stage::k_at(16 * h + i, 4 * x + g));
+    };
+    const auto read_v = [&](int b) {
 #pragma unroll
-      for (int x = 0; x < NS; x++) {
-        u32x4 f[NL];
+      for (int n = 0; n < NL; n++) fv[EARLY ? b : 0][n] = *(const u32x4 *)(C.v[n] + stage::v_at(16 * b + i, g));
+    };
+    if (EARLY) {
 #pragma unroll
-        for (int n = 0; n < NL; n++) f[n] = *(const u32x4 *)(C.k[n] + stage::k_at(16 * h + i, 4 * x + g));
+      for (int x = 0; x < NS; x++) read_k(0, x), read_k(1, x);
 #pragma unroll
-        for (int sum = 2; sum >= 0; sum--)  // the small products first
-#pragma unroll
-          for (int n = 0; n < NL; n++)
-            if (sum - n >= 0 && sum - n < 3) a[x & 1] = MFMA(f[n], qf[sum - n][x], a[x & 1]);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; r++) s[4 * h + r] = (a[0][r] + a[1][r]) * A.scale;
+      for (int b = 0; b < D / 16; b++) read_v(b);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    f32x4 a[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) a[h][0] = a[h][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int x = 0; x < NS; x++) {
+      if (!EARLY) read_k(0, x), read_k(1, x);
+#pragma unroll
+      for (int sum = 2; sum >= 0; sum--)  // the small products first
+#pragma unroll
+        for (int n = 0; n < NL; n++)
+          if (sum - n >= 0 && sum - n < 3)
+#pragma unroll
+            for (int h = 0; h < 2; h++) a[h][x & 1] = MFMA(f[h][EARLY ? x : 0][n], qf[sum - n][x], a[h][x & 1]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) s[4 * h + r] = (a[h][0][r] + a[h][1][r]) * A.scale;
     if (part) {
       const uint32_t bad = s_bad[tile % 3];
       bool poison = false;
@@ -733,14 +761,12 @@ __global__ void __launch_bounds__(512) k_tree_attend_rows(dsh_tree_attn_t A, att
     }
 #pragma unroll
     for (int b = 0; b < D / 16; b++) {
-      u32x4 f[NL];
-#pragma unroll
-      for (int n = 0; n < NL; n++) f[n] = *(const u32x4 *)(C.v[n] + stage::v_at(16 * b + i, g));
+      if (!EARLY) read_v(b);
 #pragma unroll
       for (int sum = 2; sum >= 0; sum--)
 #pragma unroll
         for (int n = 0; n < NL; n++)
-          if (sum - n >= 0 && sum - n < 3) o[b] = MFMA(f[n], pf[sum - n], o[b]);
+          if (sum - n >= 0 && sum - n < 3) o[b] = MFMA(fv[EARLY ? b : 0][n], pf[sum - n], o[b]);
     }
   };
   // one barrier a tile: tile n is read while tile n + 1 is written to the other half
