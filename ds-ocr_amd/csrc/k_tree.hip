@@ -70,9 +70,6 @@ __device__ __forceinline__ bool tree_in_window(int p, int pos, int prefill_len, 
 //   f32 cache: v_mfma_f32_16x16x4, exact products and f32 sums. bf16 cache: v_mfma_f32_16x16x32_bf16, the f32 queries and
 //   weights in three bf16 parts each that add up to them exactly (24 bits), so that only the f32 sums round.
 #define ATT_SLACK 10.0f
-#ifndef STAGED_TILES
-#define STAGED_TILES 3
-#endif
 #define ATT_L2E 1.44269504088896340736f
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -260,9 +257,11 @@ struct frag_bf16 {
 };
 
 // A block: tile_rows x pos_waves waves over one split of the tiles of one key head; the waves of a row tile put their sums
-// together, and the block writes them for k_tree_join (splits > 1) or finishes its rows itself.
-template <int D, bool BF, int W>
-__global__ void __launch_bounds__(64 * W, W == 4 && D <= 128 ? 2 : 1) k_tree_attend(dsh_tree_attn_t A, attend_plan P) {
+// together, and the block writes them for k_tree_join (splits > 1) or finishes its rows itself. Up to a few hundred rows the
+// launches and the first loads' round trips are all (5 nodes over 77 rows 8.4 us, 16 over 701 11.5 with the join's 3); then
+// the cache's bytes (10 heads x 128: 7001 rows 18.6 us for one node, 20 for 16, 72 MB; 30000 rows 61 us, 307 MB, 5.0 TB/s).
+template <int D, bool BF>
+__global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_tree_attend(dsh_tree_attn_t A, attend_plan P) {
   typedef typename std::conditional<BF, frag_bf16<D>, frag_f32<D>>::type frag;
   constexpr int AT = frag::AT, NV = AT / 4;  // scores a lane
   __shared__ tree_lds t;
@@ -458,6 +457,11 @@ __global__ void __launch_bounds__(64 * W, W == 4 && D <= 128 ? 2 : 1) k_tree_att
 // exclusive-ored so that the 16 lanes of a read or write meet all banks. The last SW waves bring the next tile into the other
 // half of the LDS while the others compute, one of each kind to a SIMD, so that the vector units' splitting and the matrix
 // units' products go on at once; where there are rows for all eight (SW = 8), each does both, half of them in the other order.
+// What bounds it is the length of a tile's steps in a wave (LDS reads, products, weights, products: 4500 cycles for 1536 of
+// products with an f32 cache, 3600 for 768 with a bf16 one): 64 nodes over 7001 rows 25 us and 5 for the
+// join, against 37 and 5 in k_tree_attend with f32 products; 24 nodes of 16 heads over 120011 bf16 rows 88 us (246 MB, 2.8
+// TB/s) and 5, against 147. Two row tiles to a wave (half the LDS reads) spill and take 43 and 150 us, 64 positions a step
+// 126 with the bf16 cache.
 template <int D, bool BF>
 struct staged {
   static constexpr int NL = BF ? 1 : 3, E = BF ? 8 : 4;  // parts; dimensions of a unit: 4 positions x E, 16 bytes a position
@@ -1258,15 +1262,18 @@ extern "C" {
       return hipErrorInvalidValue; \
   }
 
-// The cut of a launch's work. Row tiles: up to 8 (D <= 128; 4 beyond, whose registers need a whole SIMD) in a block, a wave each,
-// so that K and V come from the first-level cache for all but one of them; with fewer than 3 the rest of four waves share the
-// positions. Splits: as many as keep the card's 1024 SIMDs at two waves each, and no wave without a tile.
+// The cut of a launch's work, by measurement (10 heads x 128 and an f32 cache, or 16 x 128 over 4 bf16 ones).
+// More than one row tile: k_tree_attend_rows (32 nodes over 7001 f32 rows 25.1 us against 27.8, 8 nodes over 4000 bf16 rows 12.7
+// against 14.1); one: k_tree_attend, whose four waves share the positions (16 nodes over 7001 rows 23.1 us against 23.8). An
+// f32 cache of 192 or 256 dimensions, whose parts do not fit the LDS twice, takes k_tree_attend with up to four row tiles.
+// Splits: a block to a CU (one node over 7001 rows: 18.6 us, half as many blocks 20.1, twice as many 20.8; 64 nodes 25.2, 37 and
+// 34), but one where that leaves a wave no more than four tiles (5 nodes over 77 rows: 8.4 us; in two splits, joined, 10.7).
 static attend_plan attend_cut(const dsh_tree_attn_t *A) {
   attend_plan P;
   memset(&P, 0, sizeof P);
   const int G = A->cache.n_heads, D = A->cache.head_dim;
   const int64_t rows = (int64_t)A->n_nodes * (A->n_heads / G), row_tiles = (rows + 15) / 16;
-  P.staged = row_tiles >= STAGED_TILES && (A->cache.bf16 || D <= 128);
+  P.staged = row_tiles > 1 && (A->cache.bf16 || D <= 128);
   const int AT = A->cache.bf16 || P.staged ? 32 : 16, most = P.staged || D <= 128 ? 8 : 4;
   P.groups = (int)((row_tiles + most - 1) / most);
   P.tile_rows = (int)((row_tiles + P.groups - 1) / P.groups);
@@ -1284,9 +1291,7 @@ static attend_plan attend_cut(const dsh_tree_attn_t *A) {
     }
   }
   const int64_t tiles = (int64_t)P.cache_tiles - P.skip + P.tree_tiles;
-  // two blocks of four waves fit a CU, one of more
-  const int64_t want = (!P.staged && P.tile_rows * P.pos_waves <= 4 ? 512 : 256) / ((int64_t)G * P.groups);
-  // up to four tiles a wave cost less than a second kernel that joins splits
+  const int64_t want = 256 / ((int64_t)G * P.groups);
   int64_t splits = (tiles + P.pos_waves - 1) / P.pos_waves;
   if (splits <= 4) splits = 1;
   if (splits > want) splits = want;
@@ -1310,7 +1315,7 @@ hipError_t dsh_launch_tree_attention(const dsh_tree_attn_t *A, float *work, hipS
   if (A->n_nodes < 1 || A->n_nodes > DSH_TREE_MAX) return hipErrorInvalidValue;
   attend_plan P = attend_cut(A);
   const int D = A->cache.head_dim, W = P.tile_rows * P.pos_waves;
-  if (W > 8 || P.groups > 65535 || (P.splits > 1 && !work)) return hipErrorInvalidValue;
+  if (W > 8 || (!P.staged && W > 4) || P.groups > 65535 || (P.splits > 1 && !work)) return hipErrorInvalidValue;
   P.part = work;
   P.ml = work ? work + (size_t)A->cache.n_heads * P.groups * P.splits * 16 * P.tile_rows * D : nullptr;
   const dim3 grid(P.splits, A->cache.n_heads, P.groups);
@@ -1321,15 +1326,17 @@ hipError_t dsh_launch_tree_attention(const dsh_tree_attn_t *A, float *work, hipS
       if constexpr (BF || D <= 128) {                                                 \
         if (P.tile_rows <= 4)                                                         \
           k_tree_attend_rows<D, BF, 4><<<grid, 512, 0, s>>>(*A, P);                   \
-        else if (P.tile_rows <= 6)                                                    \
-          k_tree_attend_rows<D, BF, 2><<<grid, 512, 0, s>>>(*A, P);                   \
-        else                                                                          \
+        else if constexpr (BF) {                                                      \
+          if (P.tile_rows <= 6)                                                       \
+            k_tree_attend_rows<D, BF, 2><<<grid, 512, 0, s>>>(*A, P);                 \
+          else                                                                        \
+            k_tree_attend_rows<D, BF, 8><<<grid, 512, 0, s>>>(*A, P);                 \
+        } else                                                                        \
           k_tree_attend_rows<D, BF, 8><<<grid, 512, 0, s>>>(*A, P);                   \
       }                                                                               \
-    } else if (W <= 4)                                                                \
-      k_tree_attend<D, BF, 4><<<grid, 64 * W, lds, s>>>(*A, P);                       \
-    else                                                                              \
-      k_tree_attend<D, BF, 8><<<grid, 64 * W, lds, s>>>(*A, P);                       \
+    } else {                                                                          \
+      k_tree_attend<D, BF><<<grid, 64 * W, lds, s>>>(*A, P);                          \
+    }                                                                                 \
     if (P.splits > 1)                                                                 \
       k_tree_join<D><<<dim3(A->n_nodes * (A->n_heads / A->cache.n_heads), A->cache.n_heads), 256, 0, s>>>(*A, P); \
     break;
