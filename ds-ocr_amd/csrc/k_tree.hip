@@ -882,7 +882,9 @@ __global__ void __launch_bounds__(256) k_tree_join(dsh_tree_attn_t A, attend_pla
 // drawn from q and rejected), so what counts is the chain of dependent reads. Every block walks the tree by itself (a wave
 // holds a node a lane, twice, with the probabilities at its token fetched ahead), and owns 1/gridDim.x of the row: a sum over
 // the row is each block's share, told to all others through tagged words. The last such sum also says which block the drawn
-// token lies in, and that block finds it.
+// token lies in, and that block finds it. A chain of 5 or 64 nodes over 129280 tokens 6.3 us, 24 drawn ones 6.3 (one block that did
+// it all: 177, 226 and 221); of the kernel's 5.2 us some 1.4 are the probabilities' two round trips, 1.6 the row, 1.8 the sums'
+// way from block to block.
 
 // A probability: what is not positive and finite counts as 0.
 __device__ __forceinline__ double prob(float x) { return x > 0.0f && x < __builtin_huge_valf() ? (double)x : 0.0; }
@@ -979,7 +981,7 @@ __global__ void __launch_bounds__(VB) k_tree_verify(verify_args A) {
   __shared__ verify_lds L;
   __shared__ int s_path[DSH_TREE_MAX];
   const int n = A.n, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, blocks = gridDim.x, me = blockIdx.x;
-  const int lo = me * A.share, hi = min(lo + A.share, A.vocab);
+  const int lo = me * A.share, hi = min(lo + A.share, A.vocab);  // vocab is 2^30 at most
   // node lane and node lane + 64
   int par0 = -2, par1 = -2, tok0 = -1, tok1 = -1;
   float u0 = 0.0f, u1 = 0.0f;
@@ -1120,9 +1122,10 @@ __global__ void __launch_bounds__(VB) k_tree_verify(verify_args A) {
     if (tid == 0) {
       A.result[0] = failed ? 0 : count;
       if (failed || !(total > 0.0)) A.result[1] = -1;
-      if (failed && A.derr) __hip_atomic_store(A.derr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
     }
   }
+  // any block's: another may have come too late for the others, and then have found all of their sums
+  if (failed && tid == 0 && A.derr) __hip_atomic_store(A.derr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
   if (failed || !(total > 0.0)) return;
   // the first block whose share crosses the threshold (for a number beyond [0, 1) the last with anything in it), then the
   // wave, the lane and the value
@@ -1213,27 +1216,41 @@ __global__ void __launch_bounds__(64) k_tree_verify_greedy(int *path, int *resul
 }
 
 // ---------------------------------------------------------------------------- commit
-// Blocks (x, head): the columns [256 x, 256 x + 256) of the head's weights; the last x the rows that are new.
-template <int D, typename T>
+// Blocks (x, head): the columns [256 x, 256 x + 256) of the head's weights, a thread each, eight accepted nodes' scores at a time;
+// the last x also the rows that are new, a 16-byte piece of K or V a thread, eight rows at a time in the path's order: a path
+// ascends, path[k] >= k, so that a row is read before the one that is written over it where the tree's rows are the cache's own
+// from n_cache on. A few KB to a few MB: bound by the launch and by path, score and lse being read one after the other (4
+// nodes of 16 over 701 rows 4.2 us, 9 of 64 over 7001 5.6; one score at a time 4.7 and 7.0).
+template <int D, bool BF>
 __global__ void __launch_bounds__(256) k_tree_commit(dsh_tree_commit_t A) {
-  __shared__ int s_path[DSH_TREE_MAX], s_n;
-  const int g = blockIdx.y, n = A.n_cache, grp = A.n_heads / (A.acc ? A.cache.n_heads : 1);
-  if (threadIdx.x == 0) s_n = min(max(A.result[0], 0), A.n_nodes);
+  constexpr int P = D / (BF ? 8 : 4);  // pieces of a row
+  __shared__ int s_path[DSH_TREE_MAX];
+  const int g = blockIdx.y, n = A.n_cache, T = A.n_nodes, claimed = min(max(A.result[0], 0), T);
+  const int mine = (int)threadIdx.x < T ? A.path[threadIdx.x] : -1;
+  if ((int)threadIdx.x < T) s_path[threadIdx.x] = mine;
+  // the path ends before its first entry that is no node
+  const u64 stop = __ballot((int)threadIdx.x >= claimed || mine < 0 || mine >= T);
+  __shared__ int s_n[4];
+  if ((threadIdx.x & 63) == 0) s_n[threadIdx.x >> 6] = stop ? __builtin_ctzll(stop) : 64;
   __syncthreads();
-  if ((int)threadIdx.x < A.n_nodes) s_path[threadIdx.x] = A.path[threadIdx.x];
-  __syncthreads();
-  int count = 0;
-  while (count < s_n && s_path[count] >= 0 && s_path[count] < A.n_nodes) count++;
+  const int count = s_n[0] < 64 ? s_n[0] : 64 + s_n[1];  // two waves hold every node
   if (A.acc) {
-    const int j = blockIdx.x * 256 + threadIdx.x;
+    const int grp = A.n_heads / A.cache.n_heads, j = blockIdx.x * 256 + threadIdx.x;
     if (j < n + count) {
       const int col = j < n ? j : n + s_path[j - n];
       float a = 0.0f;
       for (int h = g * grp; h < (g + 1) * grp; h++)
-        for (int k = 0; k < count; k++) {
-          const int64_t row = (int64_t)h * A.n_nodes + s_path[k];
-          const float l = A.lse[row];
-          if (l > -__builtin_huge_valf()) a += expf(A.scores[row * A.score_stride + col] - l);
+        for (int k0 = 0; k0 < count; k0 += 8) {
+          float s[8], l[8];
+#pragma unroll
+          for (int k = 0; k < 8; k++) {
+            const int64_t row = (int64_t)h * T + s_path[min(k0 + k, count - 1)];
+            s[k] = A.scores[row * A.score_stride + col];
+            l[k] = A.lse[row];
+          }
+#pragma unroll
+          for (int k = 0; k < 8; k++)
+            if (k0 + k < count && l[k] > -__builtin_huge_valf()) a += expf(s[k] - l[k]);
         }
       const int64_t at = g * A.acc_stride + j;
       A.acc_out[at] = j < n ? A.acc[at] + a : a;
@@ -1241,12 +1258,18 @@ __global__ void __launch_bounds__(256) k_tree_commit(dsh_tree_commit_t A) {
   }
   if (blockIdx.x != gridDim.x - 1) return;
   if (A.pos && (int)threadIdx.x < count) A.pos[g * A.pos_stride + n + threadIdx.x] = A.pos0 + threadIdx.x;
-  for (int x = threadIdx.x; x < count * D; x += 256) {
-    const int k = x / D, d = x - k * D;
-    const int64_t from = s_path[k] * A.tree.row_stride + g * A.tree.head_stride + d;
-    const int64_t to = (int64_t)(n + k) * A.cache.row_stride + g * A.cache.head_stride + d;
-    ((T *)A.cache.k)[to] = ((const T *)A.tree.k)[from];
-    ((T *)A.cache.v)[to] = ((const T *)A.tree.v)[from];
+  for (int x = threadIdx.x; x < 2 * P; x += 256) {
+    constexpr int SZ = BF ? 2 : 4;
+    const char *from = (const char *)(x < P ? A.tree.k : A.tree.v) + g * A.tree.head_stride * SZ + 16 * (x < P ? x : x - P);
+    char *to = (char *)(x < P ? A.cache.k : A.cache.v) + (g * A.cache.head_stride + n * A.cache.row_stride) * SZ + 16 * (x < P ? x : x - P);
+    for (int k0 = 0; k0 < count; k0 += 8) {
+      u32x4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[k] = *(const u32x4 *)(from + s_path[min(k0 + k, count - 1)] * A.tree.row_stride * SZ);
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (k0 + k < count) *(u32x4 *)(to + (k0 + k) * A.cache.row_stride * SZ) = v[k];
+    }
   }
 }
 
@@ -1371,14 +1394,14 @@ hipError_t dsh_launch_tree_verify_greedy(int *path, int *result, const int *targ
 hipError_t dsh_launch_tree_commit(const dsh_tree_commit_t *A, hipStream_t s) {
   if (A->n_nodes < 1 || A->n_nodes > DSH_TREE_MAX) return hipErrorInvalidValue;
   const dim3 g(A->acc ? (A->n_cache + A->n_nodes + 255) / 256 : 1, A->cache.n_heads);
-#define CASE(D, T)                             \
-  case D:                                      \
-    k_tree_commit<D, T><<<g, 256, 0, s>>>(*A); \
+#define CASE(D, BF)                             \
+  case D:                                       \
+    k_tree_commit<D, BF><<<g, 256, 0, s>>>(*A); \
     break;
   if (A->cache.bf16) {
-    BY_DIM(A->cache.head_dim, uint16_t, CASE)
+    BY_DIM(A->cache.head_dim, true, CASE)
   } else {
-    BY_DIM(A->cache.head_dim, float, CASE)
+    BY_DIM(A->cache.head_dim, false, CASE)
   }
 #undef CASE
   return hipGetLastError();

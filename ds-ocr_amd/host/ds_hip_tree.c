@@ -159,7 +159,7 @@ int ds_hip_tree_verify(int *path_dev, int *result_dev, const float *p_dev, int64
   static const char *const me = "ds_hip_tree_verify";
   if (!p_dev || !u_dev) return dsr_failf("%s: NULL argument", me);
   if (verify_check(me, path_dev, result_dev, tokens_dev, parents_dev, n_nodes)) return -1;
-  if (vocab < 1 || (n_nodes > 0 && (p_stride < vocab || (q_dev && q_stride < vocab))) || p_stride > STRIDE_MAX ||
+  if (vocab < 1 || vocab > 1 << 30 || (n_nodes > 0 && (p_stride < vocab || (q_dev && q_stride < vocab))) || p_stride > STRIDE_MAX ||
       q_stride > STRIDE_MAX)
     return dsr_failf("%s: vocab %d, strides %lld and %lld", me, vocab, (long long)p_stride, (long long)q_stride);
   int dev;
@@ -246,7 +246,7 @@ int ds_hip_kv_evict(const ds_hip_kv_t *cache, int n_rows, int n_keep, const floa
                     float *acc_out_dev, int64_t acc_out_stride, const int *pos_dev, int64_t pos_stride, int *pos_out_dev,
                     int64_t pos_out_stride, int sink, int recent_from, int *slots_dev) {
   static const char *const me = "ds_hip_kv_evict";
-  if (n_rows < 0 || n_keep < 0 || n_keep > n_rows) return dsr_failf("%s: %d of %d rows", me, n_keep, n_rows);
+  if (n_rows < 0 || n_rows > 1 << 30 || n_keep < 0 || n_keep > n_rows) return dsr_failf("%s: %d of %d rows", me, n_keep, n_rows);
   if (kv_check(me, "cache", cache, n_rows)) return -1;
   if (!acc_dev) return dsr_failf("%s: NULL argument", me);
   if (pos_out_dev && !pos_dev) return dsr_failf("%s: pos_out without pos", me);

@@ -262,7 +262,8 @@ int ds_hip_attn_forward(ds_hip_attn_t *A, float *h_dev, float *n_dev, const floa
  *   per layer  ds_hip_tree_commit      the accepted nodes' K and V rows into the cache, their weights onto the rows'
  *   at need    ds_hip_kv_evict         per head the n_keep rows that stay
  * All four take device pointers, run asynchronously on the library's stream, on device 0 whatever the caller's current
- * device is, and keep nothing between calls but a grow-only workspace. Outputs must not overlap inputs unless said.
+ * device is, and keep nothing between calls but a grow-only workspace (so that they must not be called while the calling
+ * thread captures a graph of its own). Outputs must not overlap inputs unless said.
  *
  * The tree: parents_dev[i] of n_nodes (at most DS_HIP_TREE_MAX_NODES) is -1 for a child of the last committed token, or
  * the index j < i of another node. Any other value makes node i a padding node, and so is every node below one: it
@@ -311,7 +312,7 @@ int ds_hip_tree_attention(float *out_dev, int64_t out_stride, float *lse_dev, fl
  * Where no child is accepted, the step's token is drawn from what is left, w = max(p - c q, 0), or p without the rejected
  * tokens (p itself if nothing is left): the smallest v with w[v] > 0 and w[0] + ... + w[v] > u[n_nodes] * sum(w); -1 if
  * p holds nothing positive. Sums and products are in 64 bits. Tokens outside [0, vocab) are rejected; a value of p or q
- * that is not positive and finite counts as 0. path_dev[n_nodes]: the accepted nodes, then -1; result_dev[2]: their
+ * that is not positive and finite counts as 0. vocab: up to 2^30. path_dev[n_nodes]: the accepted nodes, then -1; result_dev[2]: their
  * number and the token. n_nodes 0 (tokens and parents may be NULL) draws a token from p. */
 int ds_hip_tree_verify(int *path_dev, int *result_dev, const float *p_dev, int64_t p_stride, const float *q_dev,
                        int64_t q_stride, int vocab, const int *tokens_dev, const int *parents_dev, int n_nodes,
@@ -322,7 +323,8 @@ int ds_hip_tree_verify(int *path_dev, int *result_dev, const float *p_dev, int64
 int ds_hip_tree_verify_greedy(int *path_dev, int *result_dev, const int *target_dev, const int *tokens_dev,
                               const int *parents_dev, int n_nodes);
 
-/* The accepted nodes (path_dev and result_dev[0] of a verification; entries outside [0, n_nodes) and all behind the first of
+/* tree may be the cache's own rows from n_cache on (k, v + n_cache * row_stride), for a caller that writes the drafts' rows there.
+ * The accepted nodes (path_dev and result_dev[0] of a verification; entries outside [0, n_nodes) and all behind the first of
  * them are left out) go to the rows n_cache, n_cache + 1, ... of the cache, which must hold n_cache + n_nodes rows. acc
  * (optional; [cache->n_heads][acc_stride], acc_stride >= n_cache + n_nodes): every row's attention weight so far; with
  * ds_hip_tree_attention's scores and lse of n_heads query heads,
@@ -335,7 +337,7 @@ int ds_hip_tree_commit(const ds_hip_kv_t *cache, int n_cache, const ds_hip_kv_t 
                        int n_heads, const float *acc_dev, float *acc_out_dev, int64_t acc_stride, int *pos_dev,
                        int64_t pos_stride, int pos0);
 
-/* Keeps n_keep of n_rows rows of every head, in rows 0..n_keep-1: the rows with the lowest acc go, the lower row first
+/* Keeps n_keep of n_rows rows (up to 2^30) of every head, in rows 0..n_keep-1: the rows with the lowest acc go, the lower row first
  * among equal ones (a NaN counts as -inf); rows with pos < sink or pos >= recent_from go only when no others are left
  * (pos NULL: the row number). The kept rows from n_keep on move, in order, into the evicted ones below n_keep, in order;
  * no other row is written. slots_dev (optional, [n_heads][n_keep]): the row that each one was. acc_out and pos_out

@@ -452,6 +452,32 @@ def test_commit_paths(dev, path, claimed):
     commit_case(dev, 8, 4, 2, 64, 37, path, claimed, False, in_place=True, pos=False)
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("path", [[0], [1, 2], [0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10], [1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 16, 17],
+                                  [3, 7, 20, 21, 39], list(range(5, 40))])
+def test_commit_of_rows_within_the_cache(dev, path, bf16):
+    """The drafts' rows stand in the cache itself, from n_cache on: accepted ones move down over rejected ones."""
+    L = dev.load()
+    rng = np.random.default_rng(len(path))
+    n, T, G, D = 21, 40, 2, 128
+    cache = Cache(dev, normal(rng, n + T, G, D, bf16=bf16), normal(rng, n + T, G, D, bf16=bf16), bf16)
+    want = cache.expect()
+    for w in want:
+        v = cache.view(w)
+        v[n:n + len(path)] = v[n + np.array(path)].copy()
+    size = 2 if bf16 else 4
+    st = cache.st
+    tree = dev.KvCache(st.k + n * st.row_stride * size, st.v + n * st.row_stride * size, st.row_stride, st.head_stride, T, G, D,
+                       st.dtype)
+    pth = np.array(path + [-1] * (T - len(path)), np.int32)
+    pd, rd = dev.DeviceBuffer.from_array(pth), dev.DeviceBuffer.from_array(np.array([len(path), 0], np.int32))
+    dev.check(L.ds_hip_tree_commit(cache.ref, n, C.byref(tree), T, pd.ptr, rd.ptr, None, 0, None, 0, None, None, 0, None, 0, 0),
+              "commit")
+    dev.check(L.ds_hip_sync(), "sync")
+    for got, w in zip(cache.fetch(), want):
+        same(got, w)
+
+
 # ---------------------------------------------------------------------------- eviction
 def evict_case(dev, G, D, n, keep, bf16=False, by_head=False, sink=0, recent=None, acc=None, pos=True, in_place=False, seed=0,
                outputs=True):

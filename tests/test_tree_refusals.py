@@ -85,6 +85,7 @@ def test_verification_refuses(lib):
     refused(lib, v(n=-1), "-1 nodes")
     refused(lib, v(n=129), "129 nodes")
     refused(lib, v(V=0), "vocab 0")
+    refused(lib, v(V=2 ** 30 + 1, ps=2 ** 31), "vocab")
     refused(lib, v(ps=499), "strides 499")
     refused(lib, v(q=PTR, qs=499), "499")
     g = lambda path=PTR, res=PTR, tgt=PTR, tok=PTR, par=PTR, n=4: L.ds_hip_tree_verify_greedy(path, res, tgt, tok, par, n)  # noqa: E731
@@ -122,7 +123,7 @@ def test_eviction_refuses(lib):
         a.update(o)
         return L.ds_hip_kv_evict(C.byref(a["cache"]), a["n"], a["keep"], a["acc"], a["acs"], a["out"], a["ous"], a["pos"],
                                  a["ps"], a["pout"], a["pos_s"], a["sink"], a["recent"], a["slots"])
-    for change, word in ((dict(n=-1), "-1 rows"), (dict(keep=-1), "-1 of 90"), (dict(keep=91), "91 of 90"),
+    for change, word in ((dict(n=-1), "-1 rows"), (dict(n=2 ** 30 + 1, keep=5), "rows"), (dict(keep=-1), "-1 of 90"), (dict(keep=91), "91 of 90"),
                          (dict(n=101, keep=5), "101 rows of 100"), (dict(acc=None), "NULL"), (dict(pout=PTR, pos_s=50), "pos_out"),
                          (dict(acs=89), "strides"), (dict(pos=PTR, ps=89), "strides"), (dict(out=1 << 24, ous=49), "strides"),
                          (dict(pos=PTR, ps=90, pout=1 << 24, pos_s=49), "strides"), (dict(out=PTR, ous=50), "lie apart"),
