@@ -50,13 +50,7 @@ __device__ void tree_ancestors(tree_lds &t, int up, int n) {
   if (i < n && up == -2) t.anc[i][0] = t.anc[i][1] = 0;
   __syncthreads();
 }
-__device__ __forceinline__ bool tree_bit(const u64 *anc, int a) { return (anc[a >> 6] >> (a & 63)) & 1; }
 __device__ __forceinline__ int tree_depth(const u64 *anc) { return __popcll(anc[0]) + __popcll(anc[1]) - 1; }
-
-// Whether a node at position pos sees position p (what it sees at all): R-SWA's reference positions and window.
-__device__ __forceinline__ bool tree_in_window(int p, int pos, int prefill_len, int window) {
-  return window <= 0 || pos < prefill_len || p < prefill_len || p > pos - window;
-}
 
 // ---------------------------------------------------------------------------- attention
 // The rows of one key head are the (node, query head of its group) pairs, row r node r % n_nodes of head r / n_nodes. A wave
@@ -342,20 +336,23 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_tree_attend(dsh_tree_
         s[k] = see ? s[k] : -inf;
         seen |= (uint32_t)see << k;
       }
-      // A weight of 0 does not take out a V that is not finite: such rows are set to 0, and what sees them to NaN.
-      bool poison = false;
+      // A weight of 0 does not take out a V that is not finite: such rows are set to 0, and what sees them to NaN. (At the
+      // cache's end what stands in for the rows behind it is its last row, which every node sees.)
+      if (own || A.window > 0) {
+        bool poison = false;
 #pragma unroll
-      for (int k = 0; k < NV; k++) {
-        const u64 bad = __ballot(F.clean_v(k));
-        poison |= ((bad >> (16 * g)) & 0xFFFF) && ((seen >> k) & 1);
-      }
-      if (__any(poison)) {
-        int y = poison;
-        y |= __shfl_xor(y, 16);
-        y |= __shfl_xor(y, 32);
-        if (y)
+        for (int k = 0; k < NV; k++) {
+          const u64 bad = __ballot(F.clean_v(k));
+          poison |= ((bad >> (16 * g)) & 0xFFFF) && ((seen >> k) & 1);
+        }
+        if (__any(poison)) {
+          int y = poison;
+          y |= __shfl_xor(y, 16);
+          y |= __shfl_xor(y, 32);
+          if (y)
 #pragma unroll
-          for (int b = 0; b < D / 16; b++) o[b] += __builtin_nanf("");
+            for (int b = 0; b < D / 16; b++) o[b] += __builtin_nanf("");
+        }
       }
     }
     if (sc && row < R) {
@@ -610,7 +607,7 @@ __global__ void __launch_bounds__(512) k_tree_attend_rows(dsh_tree_attn_t A, att
   // Tile t0 + n (n % AHEAD == a) to its half of the LDS, and the loads of the tile AHEAD after it.
   const auto bring = [&](int n, u32x4 (*st)[4]) {
     const where w = locate(t0 + n);
-    write(st, S[n & 1], partial(w), &s_bad[n % 3]);
+    write(st, S[n & 1], partial(w) && (w.own || A.window > 0), &s_bad[n % 3]);
     if (sid == 0) s_bad[(n + 1) % 3] = 0;  // read two tiles ago
     load(st, locate(min(t0 + n + AHEAD, tiles - 1)));
   };

@@ -46,7 +46,7 @@ int ds_hip_time_expert(const ds_int4_block_t *gate_up_int4, const ds_int4_block_
 /* Waits for the library stream. Returns -1 (message in ds_hip_last_error) if a kernel reported since
  * the last check that one of its bounded waits gave up (the prefill's down tiles waiting for their
  * gate_up tiles, the one-kernel decode layers' extra blocks waiting for the verdict on the expert
- * selection): the output of that call or step is not valid. The report is given once. */
+ * selection, a tree verification's blocks waiting for one another's sums): the output of that call or step is not valid. The report is given once. */
 int ds_hip_sync(void);
 /* Certified CFG routing (no counterpart in the reference; it makes the decode and prefill paths pick
  * exactly the experts ds_moe_router + ds_moe_top_k pick, ds_kernels.c:181-243, on the same input):

@@ -130,7 +130,9 @@ def test_attention_window(dev, n, prefill, window, bf16):
 
 @pytest.mark.parametrize("T, H, G, D, n, bf16", [(3, 10, 10, 128, 2000, False), (40, 4, 4, 128, 1500, False),
                                                  (12, 8, 2, 64, 5000, True), (70, 2, 1, 256, 900, True),
-                                                 (1, 4, 4, 128, 7679, False), (128, 2, 2, 192, 777, False)])
+                                                 (1, 4, 4, 128, 7679, False), (128, 2, 2, 192, 777, False),
+                                                 (100, 12, 2, 128, 200, False), (100, 12, 2, 64, 200, True),
+                                                 (60, 6, 1, 256, 150, False)])
 def test_attention_longer(dev, T, H, G, D, n, bf16):
     attend(dev, T, H, G, D, n, bf16, seed=T, scores=T < 40)
 
@@ -172,6 +174,29 @@ def test_attention_unseen_values(dev, what, bf16, T):
     within(out[rest], wo[rest], to[rest], "out")
     within(lse[:, rest], wl[:, rest], tl[:, rest], "lse")
     within(sc[:, rest], ws[:, rest], ts[:, rest], "scores")
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("T", [3, 30])
+def test_attention_seen_values(dev, T, bf16):
+    """A V row that is not finite and seen, the cache's last one among others: its head's outputs are not finite, the other
+    head's are right."""
+    rng = np.random.default_rng(2)
+    H, D, n = 2, 128, 77
+    parents = R.random_tree(rng, T)
+    q = normal(rng, T, H, D)
+    k, v = (normal(rng, n, H, D, bf16=bf16) for _ in range(2))
+    kt, vt = (normal(rng, T, H, D, bf16=bf16) for _ in range(2))
+    scale = float(np.float32(D ** -0.5))
+    wo, wl, ws, to, tl, ts = R.attention(q, k, v, kt, vt, n, parents, scale)
+    for row in (0, 40, n - 1):
+        cache = Cache(dev, k, v, bf16)
+        cache.view(cache.raw[1])[row, 0] = 0x7F80 if bf16 else np.inf
+        cache.bufs[1].write(cache.raw[1])
+        out, lse, sc = Attend(dev, q, cache, n, Cache(dev, kt, vt, bf16), parents, scale).call().fetch()
+        assert not np.isfinite(out[:, 0]).any()
+        within(out[:, 1], wo[:, 1], to[:, 1], "out")
+        within(lse, wl, tl, "lse")
 
 
 def test_attention_far_offsets(dev):
