@@ -513,8 +513,9 @@ __global__ void __launch_bounds__(512) k_tree_attend_rows(dsh_tree_attn_t A, att
     for (int y = 0; y < U; y++) {
       const int u = sid + SN * y;
       if (2 * UNITS % SN && u >= 2 * UNITS) continue;
-      const int x = u < UNITS ? u : u - UNITS, q = x / (D / E), c = x - q * (D / E);
-      const char *b = (u < UNITS ? w.k : w.v) + 16 * c;
+      const bool is_v = UNITS % SN ? u >= UNITS : y >= UNITS / SN;
+      const int x = is_v ? u - UNITS : u, q = x / (D / E), c = x - q * (D / E);
+      const char *b = (is_v ? w.v : w.k) + 16 * c;
       if (whole) {
         const char *p = b + w.p0 * w.rs + 4 * q * w.rs;
         st[y][0] = *(const u32x4 *)p;
@@ -532,7 +533,7 @@ __global__ void __launch_bounds__(512) k_tree_attend_rows(dsh_tree_attn_t A, att
     for (int y = 0; y < U; y++) {
       const int u = sid + SN * y;
       if (2 * UNITS % SN && u >= 2 * UNITS) continue;
-      const bool is_v = u >= UNITS;
+      const bool is_v = UNITS % SN ? u >= UNITS : y >= UNITS / SN;
       const int x = is_v ? u - UNITS : u, q = x / (D / E), c = x - q * (D / E);
       if (part && is_v) {  // what is not finite becomes 0: see k_tree_attend
 #pragma unroll
@@ -618,13 +619,21 @@ __global__ void __launch_bounds__(512) k_tree_attend_rows(dsh_tree_attn_t A, att
     __syncthreads();
     bring(0, ahead[0]);
     __syncthreads();
-    for (int n0 = 0; n0 < count; n0 += AHEAD)
+    // whole rounds, with no way past a load: a tile's write then waits for its own loads, not for those behind them too
+    int n = 1;
+    for (; n + AHEAD <= count; n += AHEAD)
 #pragma unroll
       for (int a = 0; a < AHEAD; a++) {
-        if (n0 + a >= count) break;
-        if (n0 + a + 1 < count) bring(n0 + a + 1, ahead[(a + 1) % AHEAD]);
+        bring(n + a, ahead[(a + 1) % AHEAD]);
         __syncthreads();
       }
+#pragma unroll
+    for (int a = 0; a < AHEAD; a++)
+      if (n + a < count) {
+        bring(n + a, ahead[(a + 1) % AHEAD]);
+        __syncthreads();
+      }
+    __syncthreads();
     return;
   }
   // the wave's queries, in three parts
