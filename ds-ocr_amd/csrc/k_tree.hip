@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(512) k_tree_attend_rows(dsh_tree_attn_t A, att
   typedef staged<D, BF> stage;
   constexpr int NL = stage::NL, E = stage::E, UNITS = stage::UNITS, SN = 64 * SW, U = (2 * UNITS + SN - 1) / SN, NS = D / 32;
   constexpr int AHEAD = U * (BF ? 3 : 2) <= 8 ? BF ? 3 : 2 : 1;  // tiles on their way, in registers
-  __shared__ __attribute__((aligned(16))) stage S[2];
+  __shared__ __attribute__((aligned(1024))) stage S[2];
   __shared__ uint32_t s_bad[3];  // by the tile: positions with a V that is not finite (where some row does not see all of it)
   __shared__ tree_lds t;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, g = lane >> 4;
@@ -671,17 +671,24 @@ __global__ void __launch_bounds__(512) k_tree_attend_rows(dsh_tree_attn_t A, att
     const where now = locate(t0 + tile);
     const bool own = now.own, part = partial(now);
     const int p0 = now.p0, end = now.end;
-    const stage &C = S[tile & 1];
     float s[8];
     constexpr bool EARLY = BF && D <= 128;  // all of a tile's reads from LDS ahead of their use, where registers allow
     u32x4 f[2][EARLY ? NS : 1][NL], fv[EARLY ? D / 16 : 1][NL];
+    // Places in LDS: of a row's and a dimension's first piece; the others' differ in bits, not in a sum, so an exclusive or and
+    // an immediate give them. Opaque in every tile, or each is a register for the whole loop and some of them are spilled.
+    constexpr int BITS = D % 128 ? 1 : 3;
+    uint32_t k_0 = (tile & 1) * (uint32_t)sizeof(stage) + stage::k_at(i, g);
+    uint32_t v_0 = (tile & 1) * (uint32_t)sizeof(stage) + (uint32_t)sizeof(S[0].k) + stage::v_at(i, g);
+    __asm__("" : "+v"(k_0), "+v"(v_0));
     const auto read_k = [&](int h, int x) {
+      const uint8_t *p = (const uint8_t *)S + (k_0 ^ (64 * (x & BITS))) + 64 * (x & ~BITS) + 32 * D * h;
 #pragma unroll
-      for (int n = 0; n < NL; n++) f[h][EARLY ? x : 0][n] = *(const u32x4 *)(C.k[n] + stage::k_at(16 * h + i, 4 * x + g));
+      for (int n = 0; n < NL; n++) f[h][EARLY ? x : 0][n] = *(const u32x4 *)(p + n * sizeof S[0].k[0]);
     };
     const auto read_v = [&](int b) {
+      const uint8_t *p = (const uint8_t *)S + (v_0 ^ (64 * (b & 3) + 16 * (b >> 2))) + 1024 * b;
 #pragma unroll
-      for (int n = 0; n < NL; n++) fv[EARLY ? b : 0][n] = *(const u32x4 *)(C.v[n] + stage::v_at(16 * b + i, g));
+      for (int n = 0; n < NL; n++) fv[EARLY ? b : 0][n] = *(const u32x4 *)(p + n * sizeof S[0].v[0]);
     };
     if (EARLY) {
 #pragma unroll
