@@ -454,11 +454,10 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_tree_attend(dsh_tree_
 // exclusive-ored so that the 16 lanes of a read or write meet all banks. The last SW waves bring the next tile into the other
 // half of the LDS while the others compute, one of each kind to a SIMD, so that the vector units' splitting and the matrix
 // units' products go on at once; where there are rows for all eight (SW = 8), each does both, half of them in the other order.
-// What bounds it is the length of a tile's steps in a wave (LDS reads, products, weights, products: 4500 cycles for 1536 of
-// products with an f32 cache, 3600 for 768 with a bf16 one): 64 nodes over 7001 rows 25 us and 5 for the
-// join, against 37 and 5 in k_tree_attend with f32 products; 24 nodes of 16 heads over 120011 bf16 rows 88 us (246 MB, 2.8
-// TB/s) and 5, against 147. Two row tiles to a wave (half the LDS reads) spill and take 43 and 150 us, 64 positions a step
-// 126 with the bf16 cache.
+// What bounds it is the length of a tile's steps in a wave (LDS reads, products, weights, products): 64 nodes over 7001 rows 23 us
+// and 5 for the join, against 37 and 5 in k_tree_attend with f32 products; 24 nodes of 16 heads over 120011 bf16 rows 84 us
+// (246 MB, 2.9 TB/s; 820 TFLOP/s of bf16 products) and 5, against 147. Two row tiles to a wave (half the LDS reads) spill and
+// take 43 and 150 us, 64 positions a step 126 with the bf16 cache.
 template <int D, bool BF>
 struct staged {
   static constexpr int NL = BF ? 1 : 3, E = BF ? 8 : 4;  // parts; dimensions of a unit: 4 positions x E, 16 bytes a position
@@ -619,7 +618,8 @@ __global__ void __launch_bounds__(512) k_tree_attend_rows(dsh_tree_attn_t A, att
     __syncthreads();
     bring(0, ahead[0]);
     __syncthreads();
-    // whole rounds, with no way past a load: a tile's write then waits for its own loads, not for those behind them too
+    // Whole rounds, with no way past a load: a tile's write then waits for its own loads, not for those behind them too (64
+    // nodes over 7001 f32 rows 25.5 us with the join, 27.7 with the loads behind a condition).
     int n = 1;
     for (; n + AHEAD <= count; n += AHEAD)
 #pragma unroll
@@ -675,7 +675,8 @@ __global__ void __launch_bounds__(512) k_tree_attend_rows(dsh_tree_attn_t A, att
     constexpr bool EARLY = BF && D <= 128;  // all of a tile's reads from LDS ahead of their use, where registers allow
     u32x4 f[2][EARLY ? NS : 1][NL], fv[EARLY ? D / 16 : 1][NL];
     // Places in LDS: of a row's and a dimension's first piece; the others' differ in bits, not in a sum, so an exclusive or and
-    // an immediate give them. Opaque in every tile, or each is a register for the whole loop and some of them are spilled.
+    // an immediate give them. Opaque in every tile, or each is a register for the whole loop and some of them are
+    // spilled (24 nodes of 16 heads over 120011 bf16 rows 86 us with the join, then 90; 32 over 40000 of 256 dimensions 113 and 232).
     constexpr int BITS = D % 128 ? 1 : 3;
     uint32_t k_0 = (tile & 1) * (uint32_t)sizeof(stage) + stage::k_at(i, g);
     uint32_t v_0 = (tile & 1) * (uint32_t)sizeof(stage) + (uint32_t)sizeof(S[0].k) + stage::v_at(i, g);
@@ -1299,11 +1300,11 @@ extern "C" {
   }
 
 // The cut of a launch's work, by measurement (10 heads x 128 and an f32 cache, or 16 x 128 over 4 bf16 ones).
-// More than one row tile: k_tree_attend_rows (32 nodes over 7001 f32 rows 25.1 us against 27.8, 8 nodes over 4000 bf16 rows 12.7
-// against 14.1); one: k_tree_attend, whose four waves share the positions (16 nodes over 7001 rows 23.1 us against 23.8). An
+// More than one row tile: k_tree_attend_rows (32 nodes over 7001 f32 rows 24.2 us against 24.5, 8 nodes over 4000 bf16 rows 12.8
+// against 15.0); one: k_tree_attend, whose four waves share the positions (16 nodes over 7001 rows 20.1 us against 22.0). An
 // f32 cache of 192 or 256 dimensions, whose parts do not fit the LDS twice, takes k_tree_attend with up to four row tiles.
-// Splits: a block to a CU (one node over 7001 rows: 18.6 us, half as many blocks 20.1, twice as many 20.8; 64 nodes 25.2, 37 and
-// 34), but one where that leaves a wave no more than four tiles (5 nodes over 77 rows: 8.4 us; in two splits, joined, 10.7).
+// Splits: a block to a CU (one node over 7001 rows: 18.6 us, half as many blocks 20.1, twice as many 20.8; 64 nodes 28.7, 39 and
+// 37), but one where that leaves a wave no more than four tiles (5 nodes over 77 rows: 8.4 us; in two splits, joined, 10.7).
 static attend_plan attend_cut(const dsh_tree_attn_t *A) {
   attend_plan P;
   memset(&P, 0, sizeof P);
